@@ -18,6 +18,10 @@ from csahca_amd.native import (  # noqa: F401
     dsv4_swa_decode_forward,
     hca_decode_forward,
     hybrid_decode_forward,
+    kv8_csa_decode_forward,
+    kv8_decode_forward,
+    kv8_read,
+    kv8_write,
     lib as _lib,
 )
 
@@ -34,4 +38,8 @@ __all__ = [
     "csa_decode_step",
     "hca_decode_forward",
     "hybrid_decode_forward",
+    "kv8_write",
+    "kv8_read",
+    "kv8_decode_forward",
+    "kv8_csa_decode_forward",
 ]

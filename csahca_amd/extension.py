@@ -144,3 +144,41 @@ def hybrid_decode_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     return load_cuda_extension().hybrid_decode_forward(
         q.contiguous(), k_cache.contiguous(), v_cache.contiguous(), csa_chunk_size=int(csa_chunk_size),
         csa_top_k=int(csa_top_k), hca_chunk_size=int(hca_chunk_size), csa_weight=float(csa_weight))
+
+
+# The paged 8-bit K/V cache (no reference counterpart; csahca_amd.kv8_layout).
+def kv8_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+              v_scale: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
+              counts: torch.Tensor | None = None) -> None:
+    """Quantise new tokens into the cache, in place."""
+    load_cuda_extension().kv8_write(k, v, k_cache, v_cache, k_scale, v_scale, _as(block_table, torch.int32),
+                                    _as(start, torch.int32), counts=_as_or_none(counts, torch.int32))
+
+
+def kv8_read(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+             block_table: torch.Tensor, lengths: torch.Tensor, max_tokens: int, dtype: torch.dtype = torch.bfloat16,
+             start: torch.Tensor | None = None):
+    """Read cached tokens back as [batch, kv_heads, max_tokens, head_dim] (k, v)."""
+    return load_cuda_extension().kv8_read(k_cache, v_cache, k_scale, v_scale, _as(block_table, torch.int32),
+                                          _as(lengths, torch.int32), int(max_tokens), dtype=dtype,
+                                          start=_as_or_none(start, torch.int32))
+
+
+def kv8_decode_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                       v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                       softmax_scale: float | None = None) -> torch.Tensor:
+    """Attention over all cached tokens."""
+    return load_cuda_extension().kv8_decode_forward(q.contiguous(), k_cache, v_cache, k_scale, v_scale,
+                                                    _as(block_table, torch.int32), _as(lengths, torch.int32),
+                                                    softmax_scale=softmax_scale)
+
+
+def kv8_csa_decode_forward(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                           v_scale: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                           selected_chunks: torch.Tensor, chunk_size: int,
+                           softmax_scale: float | None = None) -> torch.Tensor:
+    """CSA attention over the selected chunks of the cache."""
+    return load_cuda_extension().kv8_csa_decode_forward(q.contiguous(), k_cache, v_cache, k_scale, v_scale,
+                                                        _as(block_table, torch.int32), _as(lengths, torch.int32),
+                                                        selected_chunks.contiguous(), int(chunk_size),
+                                                        softmax_scale=softmax_scale)

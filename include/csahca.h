@@ -339,6 +339,86 @@ int csahca_dsv4_pack_tokens(const void* k_tokens, const int32_t* locs, int64_t n
                             int64_t num_pages, int64_t bytes_per_page, int64_t page_size, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* The paged 8-bit K/V cache (no reference counterpart)                       */
+/* ------------------------------------------------------------------------- */
+
+/* A cache of num_pages pages of page_size tokens (a multiple of 16, at most
+ * 256), kv_heads heads of head_dim values (a multiple of 32, at most 256):
+ *   k_cache [num_pages, kv_heads, page_size, head_dim]            1 byte a value
+ *   v_cache [num_pages, kv_heads, page_size / 16, head_dim, 16]   1 byte a value
+ *   k_scale, v_scale fp32 [num_pages, kv_heads]
+ * a value being byte * scale (both caches 16-byte aligned).  v_cache holds 16
+ * tokens of a dimension next to each other.  block_table[b, j] (int32, rows
+ * table_stride >= blocks elements apart) is the page of sequence b's tokens
+ * [j * page_size, (j + 1) * page_size); a token whose page is out of
+ * [0, num_pages) or whose block is past `blocks` is skipped: not written, not
+ * attended to, read as 0.  Scales are positive and finite; the write makes them
+ * powers of two.  Value types are float32, float16 and bfloat16. */
+enum csahca_kv8_format { CSAHCA_KV8_E4M3 = 0 /* OCP e4m3fn */, CSAHCA_KV8_INT8 = 1 };
+
+/* Quantize-on-write of new tokens.  k, v: [batch, kv_heads, new_tokens,
+ * head_dim] with element strides (batch, head, token) of their own and
+ * contiguous head_dim.  Tokens n < counts[b] (int32; NULL: all; clamped to
+ * [0, new_tokens]) of sequence b go to positions start[b] + n (int32; a
+ * negative start writes nothing).  For every page they fall in and head, K and
+ * V apart: with a = max |finite new value|, e = the least exponent in [-120,
+ * 120] with a <= L 2^e (L = 448 or 127), the scale becomes 2^e, or
+ * max(old scale, 2^e) if the page holds tokens of the sequence before start[b];
+ * if that raised it, those tokens' bytes are rounded anew at it
+ * (byte * (old / new)); the new bytes are value * (1 / scale) clamped to +-L,
+ * all rounded to nearest even.  NaN is stored as NaN in e4m3 and as 0 in int8,
+ * infinities as +-L.  Every other byte and scale stays as it was.  A page is
+ * written for one sequence of a call only. */
+int csahca_kv8_write(const void* k, const void* v, int dtype, int64_t k_stride_batch, int64_t k_stride_head,
+                     int64_t k_stride_token, int64_t v_stride_batch, int64_t v_stride_head,
+                     int64_t v_stride_token, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                     int format, int64_t num_pages, int64_t page_size, const int32_t* block_table,
+                     int64_t blocks, int64_t table_stride, const int32_t* start, const int32_t* counts,
+                     int64_t batch, int64_t kv_heads, int64_t new_tokens, int64_t head_dim, void* stream);
+
+/* Reads tokens back: k_out, v_out [batch, kv_heads, max_tokens, head_dim] hold
+ * positions start[b] + n (start NULL: 0) as byte * scale, rounded once to
+ * dtype; 0 at positions outside [0, lengths[b]) and on skipped pages. */
+int csahca_kv8_read(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int format,
+                    int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t blocks,
+                    int64_t table_stride, const int32_t* start, const int32_t* lengths, void* k_out,
+                    void* v_out, int dtype, int64_t batch, int64_t kv_heads, int64_t max_tokens,
+                    int64_t head_dim, void* stream);
+
+/* Workspace for csahca_kv8_decode_forward. */
+size_t csahca_kv8_decode_workspace_bytes(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t page_size, int64_t blocks);
+
+/* Attention over all cached tokens.  q, out: [batch, queries, heads, head_dim];
+ * head h reads K/V head h / (heads / kv_heads).  With n = lengths[b] (int32,
+ * clamped to [0, blocks * page_size]), query i of `queries` attends to tokens
+ * [0, n - queries + 1 + i): the queries are the last tokens of the sequence.
+ * out = softmax(softmax_scale q.k) V, 0 where nothing is attended to. */
+int csahca_kv8_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t queries, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
+                              const float* k_scale, const float* v_scale, int format, int64_t num_pages,
+                              int64_t page_size, const int32_t* block_table, int64_t blocks,
+                              int64_t table_stride, const int32_t* lengths, double softmax_scale,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace for csahca_kv8_csa_decode_forward. */
+size_t csahca_kv8_csa_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                             int64_t top_k, int64_t chunk_size);
+
+/* Attention over the tokens of listed chunks.  q, out: [batch, heads, head_dim];
+ * chunk_indices [batch, kv_heads, top_k] (int32 or int64), one list for the
+ * heads that share a K/V head.  Chunk c holds tokens [c * chunk_size,
+ * (c + 1) * chunk_size); ids < 0 and tokens at or past lengths[b] are skipped,
+ * a chunk listed twice counts twice; 0 when no token is left. */
+int csahca_kv8_csa_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t heads,
+                                  int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
+                                  const float* k_scale, const float* v_scale, int format, int64_t num_pages,
+                                  int64_t page_size, const int32_t* block_table, int64_t blocks,
+                                  int64_t table_stride, const int32_t* lengths, const void* chunk_indices,
+                                  int index_dtype, int64_t top_k, int64_t chunk_size, double softmax_scale,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Launch profiler (measurement aid; no counterpart in the reference)         */
 /* ------------------------------------------------------------------------- */
 
