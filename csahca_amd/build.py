@@ -33,7 +33,7 @@ TIMELINE_SOURCE = "csa_step.hip"
 ARCH = os.environ.get("CSAHCA_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["status.cpp", "csa.hip", "csa_step.hip", "dsv4.hip", "dsv4_pack.hip", "hca.hip", "block.hip",
-           "kv8_cache.hip", "kv8_attend.hip"]
+           "kv8_cache.hip", "kv8_attend.hip", "kv8_attend_e4m3.hip", "kv8_attend_int8.hip"]
 ASAN_BUILD = BUILD / "asan"
 LIB_ASAN = ASAN_BUILD / "libcsahca_asan.so"
 # Host-side sanitizers only: each -fsanitize= applies to the host compilation

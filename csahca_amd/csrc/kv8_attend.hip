@@ -1,140 +1,126 @@
-// kv8_attend.hip -- attention over the paged 8-bit K/V cache.
-#include "kv8.hpp"
+// kv8_attend.hip -- attention over the paged 8-bit K/V cache: the split, the join
+// of its parts, and the entry points.  The kernel is in kv8_attend.hpp.
+#include "kv8_attend.hpp"
 
-#include <cfloat>
+#include <algorithm>
 
 namespace csahca {
 namespace {
 
-constexpr int kThreads = 256;
-
-template <typename T>
-struct AttendArgs {
-  Kv8Cache c;
-  const T* q;
-  T* out;
-  const int32_t* lengths;
-  const void* ids;  // listed chunks, or null: all tokens
-  int64_t chunk;
-  int32_t top_k;
-  int32_t ids64;
-  int32_t queries;
-  int32_t group;  // query heads of a K/V head
-  float scale_log2;
-};
-
-__device__ __forceinline__ float block_max(float v, float* lds) {
-  v = fmaxf(v, xor_lanes(v, 32));
+// One wavefront per row (batch, K/V head, row) of a sequence that has several
+// parts: out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, M = max m_p, in
+// the order of the parts.
+template <int kPer>  // dimensions a lane
+__global__ __launch_bounds__(kKv8Threads) void kv8_join_kernel(const Kv8Attend a) {
+  const int lane = threadIdx.x % kWave;
+  const int32_t D = a.c.head_dim;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kKv8Waves + threadIdx.x / kWave;
+  const int32_t r = static_cast<int32_t>(i % a.rows);
+  const int64_t bh = i / a.rows;
+  const int32_t h = static_cast<int32_t>(bh % a.c.kv_heads);
+  const int64_t b = bh / a.c.kv_heads;
+  if (b >= a.batch) return;
+  int32_t count = 0, first = 0;
+  kv8_parts_of(a, static_cast<int32_t>(b), &count, &first);
+  if (count <= 1) return;
+  const int64_t step = static_cast<int64_t>(a.c.kv_heads) * a.rows;
+  const int64_t slot0 = (static_cast<int64_t>(first) * a.c.kv_heads + h) * a.rows + r;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  float top = -FLT_MAX;
+  for (int p = lane; p < count; p += kWave) top = fmaxf(top, ml[slot0 + p * step].x);
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v = fmaxf(v, xor_lanes(v, off));
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-  __syncthreads();
-  for (int i = 0; i < kThreads / kWave; ++i) v = fmaxf(v, lds[i]);
-  return v;
-}
-
-// One workgroup per query row (batch, query, head): kThreads token slots at a
-// time, a thread a token for the scores and a thread a dimension for the sum.
-template <typename T, typename F>
-__global__ __launch_bounds__(kThreads) void kv8_attend_row_kernel(const AttendArgs<T> a) {
-  __shared__ float q[kKv8MaxHeadDim], p[kThreads], red[kThreads / kWave];
-  __shared__ int64_t at[kThreads];
-  const Kv8Cache& c = a.c;
-  const int D = c.head_dim, heads = c.kv_heads * a.group;
-  const int64_t row = blockIdx.x;
-  const int32_t head = static_cast<int32_t>(row % heads), h = head / a.group;
-  const int32_t i = static_cast<int32_t>(row / heads % a.queries);
-  const int64_t b = row / heads / a.queries;
-  const int64_t cap = static_cast<int64_t>(c.blocks) * c.page_size;
-  int64_t n = min(max(static_cast<int64_t>(a.lengths[b]), static_cast<int64_t>(0)), cap);
-  n = n - a.queries + 1 + i;
-  const int64_t slots = a.ids ? a.top_k * a.chunk : n;
-  for (int d = threadIdx.x; d < D; d += kThreads) q[d] = to_f32(a.q[row * D + d]);
-  __syncthreads();
-  float m = -FLT_MAX, l = 0.f, o = 0.f;  // a finite start: scores that are all NaN still reach the sums
-  for (int64_t t0 = 0; t0 < slots; t0 += kThreads) {
-    const int64_t slot = t0 + threadIdx.x;
-    int64_t pos = slot;
-    if (a.ids && slot < slots) {
-      const int64_t list = (b * c.kv_heads + h) * a.top_k + slot / a.chunk;
-      const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[list] : static_cast<const int32_t*>(a.ids)[list];
-      pos = id < 0 || id > cap / a.chunk ? -1 : id * a.chunk + slot % a.chunk;
-    }
-    int32_t page = -1;
-    if (slot < slots && pos >= 0 && pos < n) page = kv8_page(c, b, pos / c.page_size);
-    float s = -__builtin_inff(), vs = 0.f;
-    int64_t base = -1;
-    if (page >= 0) {
-      const int r = static_cast<int>(pos % c.page_size);
-      const int64_t tile = kv8_tile(c, page, h);
-      const uint4* kp = reinterpret_cast<const uint4*>(c.k + tile + static_cast<int64_t>(r) * D);
-      float dot = 0.f;
-      for (int u = 0; u < D / 16; ++u) {
-        const uint4 w = kp[u];
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, xor_lanes(top, off));
+  float total = 0.f, acc[kPer];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dot = fmaf(kv8_decode<F, 0>(ww[e]), q[16 * u + 4 * e], dot);
-          dot = fmaf(kv8_decode<F, 1>(ww[e]), q[16 * u + 4 * e + 1], dot);
-          dot = fmaf(kv8_decode<F, 2>(ww[e]), q[16 * u + 4 * e + 2], dot);
-          dot = fmaf(kv8_decode<F, 3>(ww[e]), q[16 * u + 4 * e + 3], dot);
-        }
-      }
-      const int64_t sc = static_cast<int64_t>(page) * c.kv_heads + h;
-      s = dot * c.k_scale[sc] * a.scale_log2;
-      vs = c.v_scale[sc];
-      base = tile + static_cast<int64_t>(r / kKv8Group) * D * kKv8Group + r % kKv8Group;
-    }
-    const float top = fmaxf(m, block_max(s, red));
-    {
-      const float w = base >= 0 ? fast_exp2(s - top) : 0.f;
-      const float fix = fast_exp2(m - top);
-      p[threadIdx.x] = w * vs;
-      at[threadIdx.x] = base;
-      l = l * fix + w;  // this thread's slots only; the threads' sums are joined at the end
-      o *= fix;
-      m = top;
-      __syncthreads();
-      if (threadIdx.x < D) {
-        const int most = static_cast<int>(min(slots - t0, static_cast<int64_t>(kThreads)));
-        for (int t = 0; t < most; ++t)
-          if (at[t] >= 0) o = fmaf(p[t], kv8_decode<F, 0>(c.v[at[t] + threadIdx.x * kKv8Group]), o);
-      }
+  for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < count; ++p) {
+    const int64_t slot = slot0 + p * step;
+    const float2 v = ml[slot];
+    const float fix = fast_exp2(v.x - top);
+    total = fmaf(v.y, fix, total);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (lane + e * kWave < D) acc[e] = fmaf(a.part_o[slot * D + lane + e * kWave], fix, acc[e]);
+  }
+  const float inv = total != 0.f ? 1.0f / total : 0.f;
+  const int64_t heads = static_cast<int64_t>(a.c.kv_heads) * a.group;
+  const int64_t at = ((b * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) {
+    const int d = lane + e * kWave;
+    if (d >= D) continue;
+    const float y = acc[e] * inv;
+    if (a.dtype == CSAHCA_F32) {
+      static_cast<float*>(a.out)[at + d] = y;
+    } else if (a.dtype == CSAHCA_F16) {
+      static_cast<f16*>(a.out)[at + d] = from_f32<f16>(y);
+    } else {
+      static_cast<bf16*>(a.out)[at + d] = from_f32<bf16>(y);
     }
   }
-  l = wave_sum(l);
-  __syncthreads();
-  if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = l;
-  __syncthreads();
-  l = 0.f;
-  for (int w = 0; w < kThreads / kWave; ++w) l += red[w];
-  if (threadIdx.x < D) a.out[row * D + threadIdx.x] = from_f32<T>(l != 0.f ? o / l : 0.f);
 }
 
-int attend(const Kv8Cache& c, const void* q, void* out, int dtype, int format, int64_t batch, int64_t queries,
-           int64_t heads, const int32_t* lengths, const void* ids, int index_dtype, int64_t top_k, int64_t chunk,
-           double softmax_scale, hipStream_t stream) {
-  CSAHCA_REQUIRE(queries <= INT32_MAX / (batch * heads), "too many query rows in one call");
-  return dispatch_kv8_dtype(dtype, [&](auto tag) {
-    using T = decltype(tag);
-    return dispatch_kv8(format, [&](auto fmt) {
-      using F = decltype(fmt);
-      AttendArgs<T> a{c,
-                      static_cast<const T*>(q),
-                      static_cast<T*>(out),
-                      lengths,
-                      ids,
-                      chunk,
-                      static_cast<int32_t>(top_k),
-                      index_dtype == CSAHCA_I64,
-                      static_cast<int32_t>(queries),
-                      static_cast<int32_t>(heads / c.kv_heads),
-                      static_cast<float>(softmax_scale * 1.4426950408889634)};
-      return launch("kv8_attend_row_kernel", kv8_attend_row_kernel<T, F>,
-                    dim3(static_cast<uint32_t>(batch * queries * heads)), dim3(kThreads), 0, stream, a);
-    });
-  });
+// How a call is laid out over workgroups, from its sizes alone.
+struct Split {
+  int tiles;       // row tiles (16 rows) of a wavefront
+  int row_waves;   // wavefronts of a workgroup over the rows, 1, 2 or 4
+  int row_groups;
+  int min_tiles;   // 64-token tiles of a part, at least (a list: exactly)
+  int target_log2;
+  int64_t parts;   // parts over the batch, at most
+  bool joined;     // whether a sequence may have several
+};
+
+constexpr int kTargetLog2 = 9;  // workgroups that share the tokens: two a CU
+
+Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t head_dim, int64_t tiles, bool list) {
+  Split s;
+  const int most = dtype == CSAHCA_F32 || head_dim > kKv8FourTilesDim ? 2 : 4;
+  const int64_t row_tiles = ceil_div(rows, 16);
+  s.tiles = row_tiles <= 1 ? 1 : row_tiles <= 2 ? 2 : most;
+  const int64_t waves = ceil_div(row_tiles, s.tiles);
+  s.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
+  s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
+  s.target_log2 = kTargetLog2;
+  const int round = kKv8Waves / s.row_waves;
+  s.min_tiles = round;
+  const int64_t target = int64_t{1} << s.target_log2, lanes = kv_heads * s.row_groups;
+  if (list) {
+    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(tiles * batch * lanes / target + 1, round), round) * round);
+    s.parts = batch * ceil_div(tiles, s.min_tiles);
+  } else {
+    s.parts = std::min(target / lanes + batch, batch * std::max<int64_t>(ceil_div(tiles, s.min_tiles), 1));
+  }
+  s.joined = s.parts > batch;
+  return s;
+}
+
+size_t workspace_of(const Split& s, int64_t kv_heads, int64_t rows, int64_t head_dim) {
+  return s.joined ? static_cast<size_t>(s.parts * kv_heads * rows * (head_dim + 2)) * sizeof(float) : 0;
+}
+
+int attend(Kv8Attend a, int format, int64_t tiles, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  const Split s = split_of(a.dtype, a.batch, a.rows, a.c.kv_heads, a.c.head_dim, tiles, a.ids != nullptr);
+  CSAHCA_REQUIRE(s.parts <= INT32_MAX / a.c.kv_heads / s.row_groups &&
+                     a.rows <= INT32_MAX / a.c.kv_heads / a.batch,
+                 "too many query rows in one call");
+  if (s.joined && (workspace == nullptr || workspace_bytes < workspace_of(s, a.c.kv_heads, a.rows, a.c.head_dim)))
+    return fail(CSAHCA_ERR_WORKSPACE, "workspace too small for kv8 decode");
+  a.row_groups = s.row_groups;
+  a.row_waves = s.row_waves;
+  a.parts = static_cast<int32_t>(s.parts);
+  a.min_tiles = s.min_tiles;
+  a.target_log2 = s.target_log2;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + s.parts * a.c.kv_heads * a.rows * a.c.head_dim;
+  const int rc = format == CSAHCA_KV8_E4M3 ? kv8_attend_launch_e4m3(a, s.tiles, stream)
+                                           : kv8_attend_launch_int8(a, s.tiles, stream);
+  if (rc != CSAHCA_OK || !s.joined) return rc;
+  const dim3 grid(static_cast<uint32_t>(ceil_div(int64_t{a.rows} * a.c.kv_heads * a.batch, kKv8Waves)));
+  return a.c.head_dim <= 128
+             ? launch("kv8_join_kernel", kv8_join_kernel<2>, grid, dim3(kKv8Threads), 0, stream, a)
+             : launch("kv8_join_kernel", kv8_join_kernel<4>, grid, dim3(kKv8Threads), 0, stream, a);
 }
 
 int check(const Kv8Cache& c, int dtype, int format, int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads,
@@ -143,9 +129,32 @@ int check(const Kv8Cache& c, int dtype, int format, int64_t batch, int64_t queri
   CSAHCA_REQUIRE(batch >= 0 && queries >= 0 && heads >= 0, "negative dimension");
   if (const int rc = kv8_check_cache(c, format, num_pages, blocks, page_size, kv_heads, head_dim)) return rc;
   CSAHCA_REQUIRE(heads == 0 || (kv_heads > 0 && heads % kv_heads == 0), "q heads must be a multiple of the cache's heads");
-  CSAHCA_REQUIRE(batch <= INT32_MAX && queries <= INT32_MAX && heads <= 65535, "too many query rows in one call");
+  CSAHCA_REQUIRE(batch <= INT32_MAX && heads <= 65535 && (heads == 0 || queries <= INT32_MAX / heads),
+                 "too many query rows in one call");
+  CSAHCA_REQUIRE(num_pages <= INT32_MAX / (page_size / kKv8Group) / std::max<int64_t>(kv_heads, 1),
+                 "cache dimension too large");  // the kernel counts groups of 16 tokens in 32 bits
   return CSAHCA_OK;
 }
+
+Kv8Attend args_of(const Kv8Cache& c, const void* q, void* out, int dtype, int64_t batch, int64_t queries, int64_t heads,
+                  const int32_t* lengths, double softmax_scale) {
+  Kv8Attend a{};
+  a.c = c;
+  a.q = q;
+  a.out = out;
+  a.lengths = lengths;
+  a.chunk = 1;
+  a.dtype = dtype;
+  a.batch = static_cast<int32_t>(batch);
+  a.queries = static_cast<int32_t>(queries);
+  a.group = static_cast<int32_t>(heads / c.kv_heads);
+  a.rows = static_cast<int32_t>(queries * a.group);
+  a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  return a;
+}
+
+// Sub-blocks (aligned groups of 16 tokens) that a chunk of this size can touch.
+int64_t chunk_subs(int64_t chunk) { return chunk % kKv8Group == 0 ? chunk / kKv8Group : (chunk + 14) / kKv8Group + 1; }
 
 Kv8Cache cache_of(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                   int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t blocks,
@@ -156,14 +165,29 @@ Kv8Cache cache_of(const void* k_cache, const void* v_cache, const float* k_scale
                   static_cast<int32_t>(kv_heads), static_cast<int32_t>(head_dim)};
 }
 
+// The page range of a call: an empty pool holds nothing to attend to.
+int check_pool(Kv8Cache& c, const void* q, const void* out, const int32_t* lengths) {
+  CSAHCA_REQUIRE(q && out && lengths, "null tensor pointer");
+  CSAHCA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0, "q must be 16-byte aligned");
+  if (c.num_pages == 0) c.blocks = 0;
+  return c.blocks > 0 ? kv8_check_pointers(c) : static_cast<int>(CSAHCA_OK);
+}
+
 }  // namespace
 }  // namespace csahca
 
 using namespace csahca;
 
-extern "C" size_t csahca_kv8_decode_workspace_bytes(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads,
-                                                    int64_t head_dim, int64_t page_size, int64_t blocks) {
-  return 0;
+extern "C" size_t csahca_kv8_decode_workspace_bytes(int dtype, int64_t batch, int64_t queries, int64_t heads,
+                                                    int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                                    int64_t blocks) {
+  if (batch <= 0 || queries <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || page_size <= 0 || blocks < 0) return 0;
+  if (batch > INT32_MAX || heads > 65535 || queries > INT32_MAX / heads || head_dim > kKv8MaxHeadDim ||
+      page_size > kKv8MaxPage || blocks > INT32_MAX / kKv8MaxPage)
+    return 0;  // refused by the call
+  const int64_t rows = queries * (heads / kv_heads);
+  return workspace_of(split_of(dtype, batch, rows, kv_heads, head_dim, ceil_div(blocks * page_size, kKv8Tile), false),
+                      kv_heads, rows, head_dim);
 }
 
 extern "C" int csahca_kv8_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t queries,
@@ -174,23 +198,25 @@ extern "C" int csahca_kv8_decode_forward(const void* q, void* out, int dtype, in
                                          double softmax_scale, void* workspace, size_t workspace_bytes,
                                          void* stream) {
   clear_error();
-  Kv8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table, blocks,
-                        table_stride, kv_heads, head_dim);
+  Kv8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table, blocks, table_stride,
+                        kv_heads, head_dim);
   if (const int rc = check(c, dtype, format, batch, queries, heads, kv_heads, head_dim, num_pages, page_size, blocks))
     return rc;
   if (batch == 0 || queries == 0 || heads == 0) return CSAHCA_OK;
-  CSAHCA_REQUIRE(q && out && lengths, "null tensor pointer");
-  if (num_pages == 0) c.blocks = 0;  // an empty pool: nothing to attend to
-  if (c.blocks > 0) {
-    if (const int rc = kv8_check_pointers(c)) return rc;
-  }
-  return attend(c, q, out, dtype, format, batch, queries, heads, lengths, nullptr, CSAHCA_I32, 0, 1, softmax_scale,
-                static_cast<hipStream_t>(stream));
+  if (const int rc = check_pool(c, q, out, lengths)) return rc;
+  return attend(args_of(c, q, out, dtype, batch, queries, heads, lengths, softmax_scale), format,
+                ceil_div(blocks * page_size, kKv8Tile), workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t csahca_kv8_csa_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+extern "C" size_t csahca_kv8_csa_decode_workspace_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
                                                         int64_t head_dim, int64_t top_k, int64_t chunk_size) {
-  return 0;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || top_k <= 0 || chunk_size <= 0) return 0;
+  if (batch > INT32_MAX || heads > 65535 || head_dim > kKv8MaxHeadDim || chunk_size > INT32_MAX ||
+      top_k > INT32_MAX / kKv8Group / chunk_subs(chunk_size))
+    return 0;  // refused by the call
+  const int64_t rows = heads / kv_heads;
+  return workspace_of(split_of(dtype, batch, rows, kv_heads, head_dim, ceil_div(top_k * chunk_subs(chunk_size), 4), true),
+                      kv_heads, rows, head_dim);
 }
 
 extern "C" int csahca_kv8_csa_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t heads,
@@ -202,20 +228,29 @@ extern "C" int csahca_kv8_csa_decode_forward(const void* q, void* out, int dtype
                                              int64_t top_k, int64_t chunk_size, double softmax_scale,
                                              void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  Kv8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table, blocks,
-                        table_stride, kv_heads, head_dim);
+  Kv8Cache c = cache_of(k_cache, v_cache, k_scale, v_scale, num_pages, page_size, block_table, blocks, table_stride,
+                        kv_heads, head_dim);
   if (const int rc = check(c, dtype, format, batch, 1, heads, kv_heads, head_dim, num_pages, page_size, blocks))
     return rc;
   CSAHCA_REQUIRE(index_dtype == CSAHCA_I32 || index_dtype == CSAHCA_I64, "chunk_indices must be int32 or int64");
   CSAHCA_REQUIRE(chunk_size > 0, "chunk_size must be positive");
-  CSAHCA_REQUIRE(top_k >= 0 && chunk_size <= INT32_MAX && top_k <= INT32_MAX, "negative dimension");
+  CSAHCA_REQUIRE(top_k >= 0, "negative dimension");
+  CSAHCA_REQUIRE(chunk_size <= INT32_MAX && top_k <= INT32_MAX / kKv8Group / chunk_subs(chunk_size),
+                 "too many listed tokens in one call");
   if (batch == 0 || heads == 0) return CSAHCA_OK;
-  CSAHCA_REQUIRE(q && out && lengths && (chunk_indices || top_k == 0), "null tensor pointer");
-  if (num_pages == 0) c.blocks = 0;  // an empty pool: nothing to attend to
-  if (c.blocks > 0) {
-    if (const int rc = kv8_check_pointers(c)) return rc;
+  CSAHCA_REQUIRE(chunk_indices || top_k == 0, "null tensor pointer");
+  if (const int rc = check_pool(c, q, out, lengths)) return rc;
+  Kv8Attend a = args_of(c, q, out, dtype, batch, 1, heads, lengths, softmax_scale);
+  const int64_t subs = chunk_subs(chunk_size), tiles = ceil_div(top_k * subs, 4);
+  if (c.blocks > 0 && top_k > 0) {
+    a.ids = chunk_indices;
+    a.ids64 = index_dtype == CSAHCA_I64;
+    a.chunk = chunk_size;
+    a.top_k = static_cast<int32_t>(top_k);
+    a.subs = static_cast<int32_t>(subs);
+    a.list_tiles = static_cast<int32_t>(tiles);
+  } else {
+    a.c.blocks = 0;  // nothing listed: as over an empty cache
   }
-  // an empty list: a list of no chunks, told from "all tokens" by its pointer
-  return attend(c, q, out, dtype, format, batch, 1, heads, lengths, chunk_indices ? chunk_indices : lengths, index_dtype,
-                chunk_indices ? top_k : 0, chunk_size, softmax_scale, static_cast<hipStream_t>(stream));
+  return attend(a, format, a.ids ? tiles : 0, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,520 @@
+// kv8_attend.hpp -- attention over the paged 8-bit K/V cache: the kernel.
+//
+// out = softmax(c q K^T) V for R = queries * group rows of a K/V head, over the
+// tokens of a sequence or of listed chunks.  Both products are matrix
+// instructions (16x16x32, f16 operands, fp32 sums) on transposed operands:
+//
+//   S^T [64 tokens x 16 rows] = K Q^T      O^T [D x 16 rows] += V^T P^T
+//
+// so that no value changes lanes between them.  A wavefront takes 64 tokens at
+// a time, as four groups ("sub-blocks") of 16 consecutive ones.  Lane l holds
+// row n = l % 16 of the result and, for its quarter g = l / 16:
+//   * S^T: the accumulator of K tile t (t = 0..3) holds its rows 4g..4g+3.  Rows
+//     of a K tile may be any tokens, so row 4g + i of tile t is token 4t + i of
+//     sub-block g: a lane's 16 scores are the 16 tokens of its sub-block.
+//   * P^T: as the second product's operand a lane supplies 8 tokens an
+//     instruction: its sub-block's first 8 and last 8, as they stand.
+//   * V^T: the matching operand is 16 consecutive tokens of dimension
+//     16 dt + n: one 16-byte load, because the cache keeps V that way.
+//   * K: 16 bytes of a token's row a load; the order of dimensions in the sum is
+//     free, so a lane's 16 bytes feed two instructions, with q loaded alike.
+//
+// Bytes are exact in f16.  q is: its rows are scaled by a power of two to below
+// 2^15 first (bf16's range is wider than f16's; f32 goes in as two f16, 22
+// bits).  A page's K scale and the row's factor go into the score; its V scale
+// goes into the exponent: p = 2^(s + log2 vs - m) with m the running maximum of
+// that sum, so p V is in units of the largest p vs so far whatever the scales
+// are, and the softmax's sum takes p / vs.  p is rounded to 11 bits (16-bit
+// values) or 22 (f32, two f16), scaled by 2^15: f16 would lose weights below
+// 2^-14 of the largest otherwise.
+#pragma once
+
+#include <cfloat>
+
+#include "kv8.hpp"
+
+namespace csahca {
+
+constexpr int kKv8Threads = 256;
+constexpr int kKv8Waves = kKv8Threads / kWave;
+constexpr int kKv8Tile = 64;      // tokens a wavefront takes at a time
+constexpr int kKv8SegTiles = 64;  // tiles whose pages a workgroup looks up at once: a sub-block a thread
+constexpr int kKv8FourTilesDim = 128;  // head sizes up to which a wavefront holds four row tiles in registers
+constexpr float kKv8PShift = 15.0f;
+
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+struct Kv8Attend {
+  Kv8Cache c;
+  const void* q;
+  void* out;
+  const int32_t* lengths;
+  const void* ids;  // listed chunks [batch, kv_heads, top_k]; null: all tokens
+  int64_t chunk;
+  int32_t ids64;
+  int32_t top_k;
+  int32_t subs;        // sub-blocks of a chunk, at most
+  int32_t list_tiles;  // tiles of a list
+  int32_t dtype;
+  int32_t batch;
+  int32_t queries;
+  int32_t group;
+  int32_t rows;        // queries * group
+  int32_t row_groups;  // workgroups over the rows
+  int32_t row_waves;   // wavefronts of a workgroup over the rows; the others split the tokens
+  int32_t parts;       // parts of all sequences, at most
+  int32_t min_tiles;   // tiles of a part, at least
+  int32_t target_log2; // about 2^target_log2 workgroups over all
+  float scale_log2;
+  float* part_ml;      // [parts, kv_heads, rows, 2]
+  float* part_o;       // [parts, kv_heads, rows, D]
+};
+
+// Where part `part` lies: its sequence, its tiles, and how many parts the
+// sequence has (`count`, from index `first` on).
+struct Kv8Part {
+  int32_t batch, begin, end, count, first;
+};
+
+__device__ __forceinline__ int32_t kv8_length(const Kv8Attend& a, int64_t b) {
+  const int32_t cap = a.c.blocks * a.c.page_size;
+  return min(max(a.lengths[b], 0), cap);
+}
+
+__device__ __forceinline__ int32_t kv8_wave_sum(int32_t v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
+  return v;
+}
+
+__device__ __forceinline__ int32_t kv8_tiles(const Kv8Attend& a, int32_t b) {
+  return b < a.batch ? (kv8_length(a, b) + kKv8Tile - 1) / kKv8Tile : 0;
+}
+
+// Tiles of a part: one size for all sequences, from the lengths on the device,
+// so that ragged lengths spread evenly over about 2^target_log2 workgroups.
+// Whole rounds of the wavefronts that split the tokens.  Every wavefront works
+// it out by itself, a lane a sequence; `mine` is the lane's tiles of the last
+// 64 sequences (of all, where the batch is not larger).
+__device__ __forceinline__ int32_t kv8_part_size(const Kv8Attend& a, int32_t* mine) {
+  const int lane = threadIdx.x % kWave;
+  int64_t total = 0;
+  for (int base = 0; base < a.batch; base += kWave) {
+    *mine = kv8_tiles(a, base + lane);
+    total += kv8_wave_sum(*mine);
+  }
+  const int64_t per = (total * a.c.kv_heads * a.row_groups) >> a.target_log2;
+  const int32_t round = kKv8Waves / a.row_waves;
+  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + round - 1) / round * round;
+}
+
+// Inclusive prefix sum over the lanes.
+__device__ __forceinline__ int32_t kv8_wave_scan(int32_t v) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int32_t u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// The part of index `part` over all sequences, each of which has at least one
+// (batch -1: there are fewer).
+__device__ __forceinline__ Kv8Part kv8_locate(const Kv8Attend& a, int32_t part) {
+  if (a.ids) {
+    const int32_t count = (a.list_tiles + a.min_tiles - 1) / a.min_tiles, j = part % count;
+    return {part / count, j * a.min_tiles, min((j + 1) * a.min_tiles, a.list_tiles), count, part - j};
+  }
+  const int lane = threadIdx.x % kWave;
+  int32_t tiles = 0, first = 0;
+  const int32_t size = kv8_part_size(a, &tiles);
+  for (int base = 0; base < a.batch; base += kWave) {
+    if (a.batch > kWave) tiles = kv8_tiles(a, base + lane);
+    const int32_t count = base + lane < a.batch ? max((tiles + size - 1) / size, 1) : 0;
+    const int32_t upto = kv8_wave_scan(count);
+    const uint64_t hit = __ballot(first + upto > part);
+    if (hit) {
+      const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+      const int32_t n = __shfl(count, at), from = first + __shfl(upto, at) - n;
+      const int32_t j = part - from;
+      return {base + at, j * size, min((j + 1) * size, __shfl(tiles, at)), n, from};
+    }
+    first += __shfl(upto, kWave - 1);
+  }
+  return {-1, 0, 0, 0, 0};
+}
+
+// How many parts sequence b has, and the index of its first.
+__device__ __forceinline__ void kv8_parts_of(const Kv8Attend& a, int32_t b, int32_t* count, int32_t* first) {
+  if (a.ids) {
+    *count = (a.list_tiles + a.min_tiles - 1) / a.min_tiles;
+    *first = b * *count;
+    return;
+  }
+  const int lane = threadIdx.x % kWave;
+  int32_t tiles = 0;
+  const int32_t size = kv8_part_size(a, &tiles);
+  *first = 0;
+  for (int base = 0; base <= b; base += kWave) {
+    if (a.batch > kWave) tiles = kv8_tiles(a, base + lane);
+    const int32_t mine = base + lane <= b ? max((tiles + size - 1) / size, 1) : 0;
+    *first += kv8_wave_sum(mine);
+    *count = __shfl(mine, b % kWave);
+  }
+  *first -= *count;
+}
+
+// A sub-block: its index in the caches (bytes / (16 D)), its valid tokens
+// [lo, hi), its K scale and log2 of its V scale.
+struct Kv8Sub {
+  uint32_t at;
+  uint32_t lohi;
+  float ks;
+  float lv;
+};
+constexpr uint32_t kKv8Whole = 16u << 8;
+
+__device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int32_t h, int32_t n, int64_t u) {
+  const Kv8Cache& c = a.c;
+  int64_t token = u * kKv8Group;
+  int32_t lo = 0, hi = 0;
+  if (a.ids) {
+    const int64_t j = u / a.subs;
+    if (j < a.top_k) {
+      const int64_t at = (static_cast<int64_t>(b) * c.kv_heads + h) * a.top_k + j;
+      const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
+      if (id >= 0 && id <= n / a.chunk) {
+        const int64_t from = id * a.chunk, to = min(from + a.chunk, static_cast<int64_t>(n));
+        token = (from / kKv8Group + (u - j * a.subs)) * kKv8Group;
+        lo = static_cast<int32_t>(max(from - token, static_cast<int64_t>(0)));
+        hi = static_cast<int32_t>(max(min(to - token, static_cast<int64_t>(kKv8Group)), static_cast<int64_t>(0)));
+      }
+    }
+  } else {
+    hi = static_cast<int32_t>(max(min(n - token, static_cast<int64_t>(kKv8Group)), static_cast<int64_t>(0)));
+  }
+  Kv8Sub s{0u, 0u, 0.f, 0.f};
+  if (hi > lo) {
+    const int32_t block = static_cast<int32_t>(token / c.page_size);
+    const int32_t page = kv8_page(c, b, block);
+    if (page >= 0) {
+      const int32_t row = static_cast<int32_t>(token - static_cast<int64_t>(block) * c.page_size);
+      const int64_t tile = static_cast<int64_t>(page) * c.kv_heads + h;
+      s.at = static_cast<uint32_t>(tile * (c.page_size / kKv8Group) + row / kKv8Group);
+      s.lohi = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8;
+      s.ks = c.k_scale[tile];
+      s.lv = __builtin_amdgcn_logf(fmaxf(c.v_scale[tile], FLT_MIN));
+    }
+  }
+  return s;
+}
+
+// Eight bytes as eight f16.
+template <typename F>
+__device__ __forceinline__ half8_t kv8_half8(uint32_t lo, uint32_t hi) {
+  half2_t r[4];
+  if constexpr (std::is_same_v<F, E4m3>) {
+    r[0] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    r[1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    r[2] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    r[3] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+  } else {
+    // b + 128 under the exponent of 1024 is the f16 1152 + b; every step is exact
+    const half2_t off = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) - off;
+      r[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) - off;
+    }
+  }
+  return half8_t{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+}
+
+template <int D, typename F, int NP, int NT>
+__global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend a) {
+  constexpr int kSteps = D / 32;           // matrix instructions over D
+  constexpr int kWide = D / 64;            // 16-byte loads of a K row
+  constexpr bool kTail = D % 64 != 0;      // and one of 8 bytes
+  constexpr int kDTiles = D / 16;
+  constexpr int kRowPad = D + 4;
+  constexpr size_t kMergeBytes = sizeof(float) * kKv8Waves * 16 * kRowPad;
+  constexpr size_t kSubBytes = sizeof(Kv8Sub) * kKv8SegTiles * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kMergeBytes > kSubBytes ? kMergeBytes : kSubBytes];
+  __shared__ float lds_ml[kKv8Waves][16][2];
+  Kv8Sub* subs = reinterpret_cast<Kv8Sub*>(lds);
+
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int n = lane % 16, g = lane / 16;
+  uint32_t x = blockIdx.x;
+  const int32_t h = x % a.c.kv_heads;
+  x /= a.c.kv_heads;
+  const int32_t rg = x % a.row_groups, part_index = x / a.row_groups;
+  const Kv8Part part = kv8_locate(a, part_index);
+  if (part.batch < 0) return;  // fewer parts than the launch allows for
+  const int32_t b = part.batch;
+  const int32_t len = kv8_length(a, b);
+  const int32_t token_waves = kKv8Waves / a.row_waves;
+  const int32_t row0 = (rg * a.row_waves + wave / token_waves) * (NT * 16);
+  const int32_t heads = a.c.kv_heads * a.group;
+
+  // q: the lane's dimensions of row n of each row tile, in f16
+  half8_t q[NT][NP][kSteps];
+  float rc[NT], m[NT], l[NT];
+  int32_t limit[NT];  // tokens the row sees
+  f32x4_t o[NT][kDTiles];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int32_t r = min(row0 + nt * 16 + n, a.rows - 1);
+    const int32_t qi = r / a.group;
+    const int64_t at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + r % a.group) * D;
+    limit[nt] = max(len - a.queries + 1 + qi, 0);
+    float v[kSteps][8], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int d = kTail && k == kSteps - 1 ? kWide * 64 + g * 8 : k / 2 * 64 + g * 16 + k % 2 * 8;
+      if (a.dtype == CSAHCA_F32) {
+        load16(static_cast<const float*>(a.q) + at + d, v[k]);
+        load16(static_cast<const float*>(a.q) + at + d + 4, v[k] + 4);
+      } else if (a.dtype == CSAHCA_F16) {
+        load16(static_cast<const f16*>(a.q) + at + d, v[k]);
+      } else {
+        load16(static_cast<const bf16*>(a.q) + at + d, v[k]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+    }
+    top = fmaxf(top, xor_lanes(top, 16));
+    top = fmaxf(top, xor_lanes(top, 32));
+    int e2 = 15;
+    if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = __builtin_ldexpf(v[k][e], 15 - e2);
+        q[nt][0][k][e] = static_cast<_Float16>(y);
+        if constexpr (NP == 2) q[nt][1][k][e] = static_cast<_Float16>(y - static_cast<float>(q[nt][0][k][e]));
+      }
+    rc[nt] = __builtin_ldexpf(a.scale_log2, e2 - 15);
+    m[nt] = -FLT_MAX;  // finite: a row of NaN scores still reaches the sums
+    l[nt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  int32_t end = part.end;
+  if (!a.ids) {  // the last row of the workgroup sees the most
+    const int32_t last = min((rg + 1) * a.row_waves * NT * 16, a.rows) - 1;
+    end = min(end, (max(len - a.queries + 1 + last / a.group, 0) + kKv8Tile - 1) / kKv8Tile);
+  }
+  const int32_t least = len - a.queries + 1 + row0 / a.group;  // the wavefront's first row sees the least
+  const uint8_t* kbase = a.c.k + (lane % 4) * D + g * 16;
+  const uint8_t* ktail = a.c.k + (lane % 4) * D + kWide * 64 + g * 8;
+  const uint8_t* vbase = a.c.v + n * kKv8Group;
+
+  for (int32_t seg = part.begin; seg < end; seg += kKv8SegTiles) {
+    __syncthreads();
+    subs[threadIdx.x] = kv8_resolve(a, b, h, len, static_cast<int64_t>(seg) * 4 + threadIdx.x);
+    __syncthreads();
+    const int32_t seg_end = min(end - seg, kKv8SegTiles);
+    for (int32_t tile = wave % token_waves; tile < seg_end; tile += token_waves) {
+      const Kv8Sub sub = subs[tile * 4 + g];
+      const int64_t koff = static_cast<int64_t>(subs[tile * 4 + n / 4].at) * (kKv8Group * D);
+      const int64_t voff = static_cast<int64_t>(sub.at) * (kKv8Group * D);
+      uint4 kw[4][kWide > 0 ? kWide : 1];
+      uint2 kt[4];
+      uint4 vw[kDTiles];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int w = 0; w < kWide; ++w) kw[t][w] = load_global_u4(kbase + koff + 4 * t * D + 64 * w);
+        if constexpr (kTail) kt[t] = load_global_u2(ktail + koff + 4 * t * D);
+      }
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = load_global_u4(vbase + voff + dt * 16 * kKv8Group);
+
+      f32x4_t s[NT][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          half8_t ka;
+          if (kTail && k == kSteps - 1) {
+            ka = kv8_half8<F>(kt[t].x, kt[t].y);
+          } else if (k % 2 == 0) {
+            ka = kv8_half8<F>(kw[t][k / 2].x, kw[t][k / 2].y);
+          } else {
+            ka = kv8_half8<F>(kw[t][k / 2].z, kw[t][k / 2].w);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+              s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[nt][p][k], s[nt][t], 0, 0, 0);
+        }
+      }
+
+      const int32_t lo = sub.lohi & 0xff, hi = sub.lohi >> 8;
+      const int32_t token = (seg + tile) * kKv8Tile + g * kKv8Group;
+      const bool edge = __ballot(sub.lohi != kKv8Whole) != 0 || (!a.ids && (seg + tile + 1) * kKv8Tile > least);
+      if (edge) {
+        // bytes behind the sequence may be NaN, which a weight of 0 does not hide
+        uint32_t keep[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          keep[w] = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * w + e >= lo && 4 * w + e < hi) keep[w] |= 0xffu << (8 * e);
+        }
+#pragma unroll
+        for (int dt = 0; dt < kDTiles; ++dt) {
+          vw[dt].x &= keep[0];
+          vw[dt].y &= keep[1];
+          vw[dt].z &= keep[2];
+          vw[dt].w &= keep[3];
+        }
+      }
+      const float inv_vs = fast_exp2(-sub.lv);
+      half8_t pa[NT][NP][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float c = sub.ks * rc[nt];
+        float sc[16], top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] = fmaf(s[nt][i / 4][i % 4], c, sub.lv);
+        if (edge) {
+          const int32_t to = a.ids ? hi : min(hi, limit[nt] - token);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = i >= lo && i < to ? sc[i] : -__builtin_inff();
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
+        top = fmaxf(top, xor_lanes(top, 16));
+        top = fmaxf(top, xor_lanes(top, 32));
+        top = fmaxf(top, m[nt]);
+        if (__ballot(top > m[nt])) {
+          const float fix = fast_exp2(m[nt] - top);
+          l[nt] *= fix;
+#pragma unroll
+          for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] *= fix;
+          m[nt] = top;
+        }
+        const float base = m[nt] - kKv8PShift;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = fast_exp2(sc[i] - base);
+          sum += p;
+          pa[nt][0][i / 8][i % 8] = static_cast<_Float16>(p);
+          if constexpr (NP == 2)
+            pa[nt][1][i / 8][i % 8] = static_cast<_Float16>(p - static_cast<float>(pa[nt][0][i / 8][i % 8]));
+        }
+        l[nt] = fmaf(sum, inv_vs, l[nt]);
+      }
+#pragma unroll
+      for (int dt = 0; dt < kDTiles; ++dt) {
+        const half8_t v0 = kv8_half8<F>(vw[dt].x, vw[dt].y), v1 = kv8_half8<F>(vw[dt].z, vw[dt].w);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pa[nt][p][0], o[nt][dt], 0, 0, 0);
+            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pa[nt][p][1], o[nt][dt], 0, 0, 0);
+          }
+      }
+    }
+  }
+
+  // The wavefronts that split the tokens are joined, a row tile at a time.
+  float* merge = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float sum = l[nt];
+    sum += xor_lanes(sum, 16);
+    sum += xor_lanes(sum, 32);
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+      *reinterpret_cast<f32x4_t*>(merge + (wave * 16 + n) * kRowPad + dt * 16 + g * 4) = o[nt][dt];
+    if (g == 0) {
+      lds_ml[wave][n][0] = m[nt];
+      lds_ml[wave][n][1] = sum;
+    }
+    __syncthreads();
+    // thread: (row wavefront, row, four dimensions)
+    for (int i = threadIdx.x; i < a.row_waves * 16 * (D / 4); i += kKv8Threads) {
+      const int d = i % (D / 4) * 4, row = i / (D / 4) % 16, w0 = i / (D / 4 * 16) * token_waves;
+      const int32_t r = (rg * a.row_waves + w0 / token_waves) * (NT * 16) + nt * 16 + row;
+      if (r >= a.rows) continue;
+      float top = -FLT_MAX, total = 0.f;
+      for (int w = 0; w < token_waves; ++w) top = fmaxf(top, lds_ml[w0 + w][row][0]);
+      f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < token_waves; ++w) {
+        const float fix = fast_exp2(lds_ml[w0 + w][row][0] - top);
+        total = fmaf(lds_ml[w0 + w][row][1], fix, total);
+        acc += *reinterpret_cast<const f32x4_t*>(merge + ((w0 + w) * 16 + row) * kRowPad + d) * fix;
+      }
+      if (part.count > 1) {
+        const int64_t slot = (static_cast<int64_t>(part_index) * a.c.kv_heads + h) * a.rows + r;
+        *reinterpret_cast<f32x4_t*>(a.part_o + slot * D + d) = acc;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, total);
+      } else {
+        const float inv = total != 0.f ? 1.0f / total : 0.f;
+        const int64_t at =
+            ((static_cast<int64_t>(b) * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = acc[e] * inv;
+          if (a.dtype == CSAHCA_F32) {
+            static_cast<float*>(a.out)[at + e] = y;
+          } else if (a.dtype == CSAHCA_F16) {
+            static_cast<f16*>(a.out)[at + e] = from_f32<f16>(y);
+          } else {
+            static_cast<bf16*>(a.out)[at + e] = from_f32<bf16>(y);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Launch for one format; `tiles` row tiles (16 rows) a wavefront.
+template <typename F>
+int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.parts) * a.row_groups * a.c.kv_heads));
+  const auto go = [&](auto kernel) {
+    return launch("kv8_attend_kernel", kernel, grid, dim3(kKv8Threads), 0, stream, a);
+  };
+  const auto by_tiles = [&](auto dim) {
+    constexpr int D = decltype(dim)::value;
+    if (a.dtype == CSAHCA_F32) {
+      return tiles == 1 ? go(kv8_attend_kernel<D, F, 2, 1>) : go(kv8_attend_kernel<D, F, 2, 2>);
+    }
+    if constexpr (D <= kKv8FourTilesDim) {
+      if (tiles == 4) return go(kv8_attend_kernel<D, F, 1, 4>);
+    }
+    return tiles == 1 ? go(kv8_attend_kernel<D, F, 1, 1>) : go(kv8_attend_kernel<D, F, 1, 2>);
+  };
+  switch (a.c.head_dim / 32) {
+    case 1: return by_tiles(std::integral_constant<int, 32>{});
+    case 2: return by_tiles(std::integral_constant<int, 64>{});
+    case 3: return by_tiles(std::integral_constant<int, 96>{});
+    case 4: return by_tiles(std::integral_constant<int, 128>{});
+    case 5: return by_tiles(std::integral_constant<int, 160>{});
+    case 6: return by_tiles(std::integral_constant<int, 192>{});
+    case 7: return by_tiles(std::integral_constant<int, 224>{});
+    default: return by_tiles(std::integral_constant<int, 256>{});
+  }
+}
+
+int kv8_attend_launch_e4m3(const Kv8Attend& a, int tiles, hipStream_t stream);
+int kv8_attend_launch_int8(const Kv8Attend& a, int tiles, hipStream_t stream);
+
+}  // namespace csahca

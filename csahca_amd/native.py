@@ -86,10 +86,10 @@ _SIGNATURES = {
                                 _vp] + [_i64] * 4 + [_vp]),
     "csahca_kv8_read": (_int, [_vp] * 4 + [_int, _i64, _i64, _vp, _i64, _i64] + [_vp] * 4 + [_int] + [_i64] * 4 +
                         [_vp]),
-    "csahca_kv8_decode_workspace_bytes": (_sz, [_i64] * 7),
+    "csahca_kv8_decode_workspace_bytes": (_sz, [_int] + [_i64] * 7),
     "csahca_kv8_decode_forward": (_int, [_vp, _vp, _int] + [_i64] * 5 + [_vp] * 4 + [_int, _i64, _i64, _vp, _i64,
                                          _i64, _vp, _dbl, _vp, _sz, _vp]),
-    "csahca_kv8_csa_decode_workspace_bytes": (_sz, [_i64] * 6),
+    "csahca_kv8_csa_decode_workspace_bytes": (_sz, [_int] + [_i64] * 6),
     "csahca_kv8_csa_decode_forward": (_int, [_vp, _vp, _int] + [_i64] * 4 + [_vp] * 4 + [_int, _i64, _i64, _vp, _i64,
                                              _i64, _vp, _vp, _int, _i64, _i64, _dbl, _vp, _sz, _vp]),
     "csahca_profile_begin": (_int, []),
@@ -1284,7 +1284,7 @@ def kv8_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     queries = q.shape[1] if q.dim() == 4 else 1
     H, page, blocks = k_cache.shape[1], k_cache.shape[2], block_table.shape[1]
     out = torch.empty_like(q)
-    nbytes = _ws_bytes("csahca_kv8_decode_workspace_bytes", B, queries, heads, H, D, page, blocks)
+    nbytes = _ws_bytes("csahca_kv8_decode_workspace_bytes", _DTYPES[q.dtype], B, queries, heads, H, D, page, blocks)
     ws = _workspace(nbytes, q.device) if nbytes else None
     rc = lib().csahca_kv8_decode_forward(
         q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, queries, heads, H, D,
@@ -1319,7 +1319,7 @@ def kv8_csa_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, l
     B, heads, D = q.shape
     H, top_k = k_cache.shape[1], chunk_indices.shape[2]
     out = torch.empty_like(q)
-    nbytes = _ws_bytes("csahca_kv8_csa_decode_workspace_bytes", B, heads, H, D, top_k, chunk_size)
+    nbytes = _ws_bytes("csahca_kv8_csa_decode_workspace_bytes", _DTYPES[q.dtype], B, heads, H, D, top_k, chunk_size)
     ws = _workspace(nbytes, q.device) if nbytes else None
     rc = lib().csahca_kv8_csa_decode_forward(
         q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, heads, H, D,

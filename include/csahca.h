@@ -386,8 +386,9 @@ int csahca_kv8_read(const void* k_cache, const void* v_cache, const float* k_sca
                     int64_t head_dim, void* stream);
 
 /* Workspace for csahca_kv8_decode_forward. */
-size_t csahca_kv8_decode_workspace_bytes(int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads,
-                                         int64_t head_dim, int64_t page_size, int64_t blocks);
+size_t csahca_kv8_decode_workspace_bytes(int dtype, int64_t batch, int64_t queries, int64_t heads,
+                                         int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                         int64_t blocks);
 
 /* Attention over all cached tokens.  q, out: [batch, queries, heads, head_dim];
  * head h reads K/V head h / (heads / kv_heads).  With n = lengths[b] (int32,
@@ -402,8 +403,8 @@ int csahca_kv8_decode_forward(const void* q, void* out, int dtype, int64_t batch
                               void* workspace, size_t workspace_bytes, void* stream);
 
 /* Workspace for csahca_kv8_csa_decode_forward. */
-size_t csahca_kv8_csa_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                                             int64_t top_k, int64_t chunk_size);
+size_t csahca_kv8_csa_decode_workspace_bytes(int dtype, int64_t batch, int64_t heads, int64_t kv_heads,
+                                             int64_t head_dim, int64_t top_k, int64_t chunk_size);
 
 /* Attention over the tokens of listed chunks.  q, out: [batch, heads, head_dim];
  * chunk_indices [batch, kv_heads, top_k] (int32 or int64), one list for the

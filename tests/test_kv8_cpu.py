@@ -96,12 +96,20 @@ def test_other_argument_errors_before_any_launch(lib):
 
 def test_workspace_sizes(lib):
     big = 1 << 40
-    assert lib.csahca_kv8_decode_workspace_bytes(-1, 1, 8, 8, 128, 64, 8) == 0
-    assert lib.csahca_kv8_decode_workspace_bytes(1, 1, 8, 0, 128, 64, 8) == 0
-    assert lib.csahca_kv8_csa_decode_workspace_bytes(1, 8, 0, 128, 8, 64) == 0
-    assert lib.csahca_kv8_csa_decode_workspace_bytes(1, 8, 8, 128, -8, 64) == 0
-    lib.csahca_kv8_decode_workspace_bytes(big, big, big, 1, 128, 64, big)
-    lib.csahca_kv8_csa_decode_workspace_bytes(big, big, 1, 128, big, big)
+    f, g = lib.csahca_kv8_decode_workspace_bytes, lib.csahca_kv8_csa_decode_workspace_bytes
+    assert f(2, -1, 1, 8, 8, 128, 64, 8) == f(2, 1, 1, 8, 0, 128, 64, 8) == f(2, 0, 1, 8, 8, 128, 64, 8) == 0
+    assert g(2, 1, 8, 0, 128, 8, 64) == g(2, 1, 8, 8, 128, -8, 64) == g(2, 1, 8, 8, 128, 0, 64) == 0
+    assert f(2, 1, 1, 8, 8, 128, 64, 1) == 0  # one part a sequence: nothing to join
+    # parts of at least 4 tiles of 64 tokens: 32 for 8192 tokens, each a row of 128 values, a maximum and a sum
+    assert f(2, 1, 1, 8, 8, 128, 64, 128) == 32 * 8 * 130 * 4
+    assert f(2, big, big, big, 1, 128, 64, big) == 0 and g(2, big, big, 1, 128, big, big) == 0
+    assert f(0, 4, 50, 64, 8, 256, 256, 4096) > 0 and g(2, 32, 8, 8, 128, 32, 64) > 0
+
+
+def test_missing_workspace_is_reported(lib):
+    assert _attend(lib, blocks=128, tstride=128) == 2 and "workspace too small" in _error(lib)
+    assert _csa(lib, top_k=64) == 2 and "workspace too small" in _error(lib)
+    assert _attend(lib, q=8) == 1 and "16-byte aligned" in _error(lib)
 
 
 def test_binding_rejects_cpu_tensors():
