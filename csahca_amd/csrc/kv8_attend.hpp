@@ -38,7 +38,8 @@ namespace csahca {
 constexpr int kKv8Threads = 256;
 constexpr int kKv8Waves = kKv8Threads / kWave;
 constexpr int kKv8Tile = 64;      // tokens a wavefront takes at a time
-constexpr int kKv8SegTiles = 64;  // tiles whose pages a workgroup looks up at once: a sub-block a thread
+constexpr int kKv8SegTiles = 256;  // tiles whose pages a workgroup looks up at once
+constexpr int kKv8Lookups = kKv8SegTiles * 4 / kKv8Threads;  // sub-blocks of a segment a thread
 constexpr int kKv8FourTilesDim = 128;  // head sizes up to which a wavefront holds four row tiles in registers
 constexpr float kKv8PShift = 15.0f;
 
@@ -67,6 +68,7 @@ struct Kv8Attend {
   int32_t parts;       // parts of all sequences, at most
   int32_t min_tiles;   // tiles of a part, at least
   int32_t target_log2; // about 2^target_log2 workgroups over all
+  int32_t join_lanes;  // of a joining workgroup, thread groups that share a row's parts
   float scale_log2;
   float* part_ml;      // [parts, kv_heads, rows, 2]
   float* part_o;       // [parts, kv_heads, rows, D]
@@ -168,12 +170,11 @@ __device__ __forceinline__ void kv8_parts_of(const Kv8Attend& a, int32_t b, int3
 }
 
 // A sub-block: its index in the caches (bytes / (16 D)), its valid tokens
-// [lo, hi), its K scale and log2 of its V scale.
+// [lo, hi), and the index of its scales (-1: no valid token).
 struct Kv8Sub {
   uint32_t at;
   uint32_t lohi;
-  float ks;
-  float lv;
+  int32_t scale;
 };
 constexpr uint32_t kKv8Whole = 16u << 8;
 
@@ -182,7 +183,7 @@ __device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int
   int64_t token = u * kKv8Group;
   int32_t lo = 0, hi = 0;
   if (a.ids) {
-    const int64_t j = u / a.subs;
+    const int64_t j = static_cast<int32_t>(u) / a.subs;
     if (j < a.top_k) {
       const int64_t at = (static_cast<int64_t>(b) * c.kv_heads + h) * a.top_k + j;
       const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
@@ -196,17 +197,15 @@ __device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int
   } else {
     hi = static_cast<int32_t>(max(min(n - token, static_cast<int64_t>(kKv8Group)), static_cast<int64_t>(0)));
   }
-  Kv8Sub s{0u, 0u, 0.f, 0.f};
+  Kv8Sub s{0u, 0u, -1};
   if (hi > lo) {
-    const int32_t block = static_cast<int32_t>(token / c.page_size);
+    const int32_t block = static_cast<int32_t>(token) / c.page_size;
     const int32_t page = kv8_page(c, b, block);
     if (page >= 0) {
-      const int32_t row = static_cast<int32_t>(token - static_cast<int64_t>(block) * c.page_size);
-      const int64_t tile = static_cast<int64_t>(page) * c.kv_heads + h;
-      s.at = static_cast<uint32_t>(tile * (c.page_size / kKv8Group) + row / kKv8Group);
+      const int32_t row = static_cast<int32_t>(token) - block * c.page_size;
+      s.scale = page * c.kv_heads + h;
+      s.at = static_cast<uint32_t>(s.scale * (c.page_size / kKv8Group) + row / kKv8Group);
       s.lohi = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8;
-      s.ks = c.k_scale[tile];
-      s.lv = __builtin_amdgcn_logf(fmaxf(c.v_scale[tile], FLT_MIN));
     }
   }
   return s;
@@ -234,6 +233,20 @@ __device__ __forceinline__ half8_t kv8_half8(uint32_t lo, uint32_t hi) {
   return half8_t{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
+// Four values to the output, rounded to its type.
+__device__ __forceinline__ void kv8_store4(const Kv8Attend& a, int64_t at, f32x4_t y) {
+  if (a.dtype == CSAHCA_F32) {
+    *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = y;
+  } else {
+    uint16_t r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      r[e] = a.dtype == CSAHCA_F16 ? __builtin_bit_cast(uint16_t, static_cast<f16>(y[e])) : float_to_bf16_bits(y[e]);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+        make_uint2(r[0] | static_cast<uint32_t>(r[1]) << 16, r[2] | static_cast<uint32_t>(r[3]) << 16);
+  }
+}
+
 template <int D, typename F, int NP, int NT>
 __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend a) {
   constexpr int kSteps = D / 32;           // matrix instructions over D
@@ -242,10 +255,11 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
   constexpr int kDTiles = D / 16;
   constexpr int kRowPad = D + 4;
   constexpr size_t kMergeBytes = sizeof(float) * kKv8Waves * 16 * kRowPad;
-  constexpr size_t kSubBytes = sizeof(Kv8Sub) * kKv8SegTiles * 4;
+  constexpr size_t kSubBytes = 16 * kKv8SegTiles * 4;
   __shared__ __attribute__((aligned(16))) char lds[kMergeBytes > kSubBytes ? kMergeBytes : kSubBytes];
   __shared__ float lds_ml[kKv8Waves][16][2];
-  Kv8Sub* subs = reinterpret_cast<Kv8Sub*>(lds);
+  uint2* sub_at = reinterpret_cast<uint2*>(lds);                          // index, valid tokens
+  float2* sub_scale = reinterpret_cast<float2*>(lds) + kKv8SegTiles * 4;  // K scale, log2 of the V scale
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = lane % 16, g = lane / 16;
@@ -261,28 +275,97 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
   const int32_t row0 = (rg * a.row_waves + wave / token_waves) * (NT * 16);
   const int32_t heads = a.c.kv_heads * a.group;
 
-  // q: the lane's dimensions of row n of each row tile, in f16
-  half8_t q[NT][NP][kSteps];
-  float rc[NT], m[NT], l[NT];
+  // The lane's dimensions of row n of each row tile, as they are stored.
+  u32x4_t raw[NT][kSteps][NP];
   int32_t limit[NT];  // tokens the row sees
-  f32x4_t o[NT][kDTiles];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int32_t r = min(row0 + nt * 16 + n, a.rows - 1);
     const int32_t qi = r / a.group;
     const int64_t at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + r % a.group) * D;
     limit[nt] = max(len - a.queries + 1 + qi, 0);
-    float v[kSteps][8], top = 0.f;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const int d = kTail && k == kSteps - 1 ? kWide * 64 + g * 8 : k / 2 * 64 + g * 16 + k % 2 * 8;
-      if (a.dtype == CSAHCA_F32) {
-        load16(static_cast<const float*>(a.q) + at + d, v[k]);
-        load16(static_cast<const float*>(a.q) + at + d + 4, v[k] + 4);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        raw[nt][k][p] = load_global_raw<u32x4_t>(static_cast<const uint8_t*>(a.q) + (at + d) * 2 * NP + 16 * p);
+    }
+  }
+
+  int32_t end = part.end;
+  if (!a.ids) {  // the last row of the workgroup sees the most
+    const int32_t last = min((rg + 1) * a.row_waves * NT * 16, a.rows) - 1;
+    end = min(end, (max(len - a.queries + 1 + last / a.group, 0) + kKv8Tile - 1) / kKv8Tile);
+  }
+  const int32_t least = len - a.queries + 1 + row0 / a.group;  // the wavefront's first row sees the least
+  const uint8_t* kbase = a.c.k + (lane % 4) * D + g * 16;
+  const uint8_t* ktail = a.c.k + (lane % 4) * D + kWide * 64 + g * 8;
+  const uint8_t* vbase = a.c.v + n * kKv8Group;
+
+  uint4 kw[4][kWide > 0 ? kWide : 1];
+  uint2 kt[4];
+  uint4 vw[kDTiles];
+  const auto load_k = [&](uint32_t at) {
+    const int64_t off = static_cast<int64_t>(at) * (kKv8Group * D);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int w = 0; w < kWide; ++w) kw[t][w] = load_global_u4(kbase + off + 4 * t * D + 64 * w);
+      if constexpr (kTail) kt[t] = load_global_u2(ktail + off + 4 * t * D);
+    }
+  };
+  const auto load_v = [&](uint32_t at) {
+    const int64_t off = static_cast<int64_t>(at) * (kKv8Group * D);
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = load_global_u4(vbase + off + dt * 16 * kKv8Group);
+  };
+
+  // The pages of the segment's sub-blocks, then this wavefront's first loads and
+  // the sub-blocks' scales, which only the scores wait for.
+  float ks[kKv8Lookups], vs[kKv8Lookups];
+  const int32_t first = wave % token_waves;
+  const auto look_up = [&](int32_t seg, int32_t tiles) {
+#pragma unroll
+    for (int i = 0; i < kKv8Lookups; ++i) {
+      const int at = i * kKv8Threads + threadIdx.x;
+      ks[i] = 0.f;
+      vs[i] = 1.f;
+      if (at < tiles * 4) {
+        const Kv8Sub sub = kv8_resolve(a, b, h, len, static_cast<int64_t>(seg) * 4 + at);
+        sub_at[at] = make_uint2(sub.at, sub.lohi);
+        if (sub.scale >= 0) {
+          ks[i] = a.c.k_scale[sub.scale];
+          vs[i] = a.c.v_scale[sub.scale];
+        }
+      }
+    }
+    lds_barrier();
+    if (first < tiles) {
+      load_k(sub_at[first * 4 + n / 4].x);
+      load_v(sub_at[first * 4 + g].x);
+    }
+  };
+  look_up(part.begin, min(end - part.begin, kKv8SegTiles));
+
+  // q in f16, its rows scaled to below 2^15
+  half8_t q[NT][NP][kSteps];
+  float rc[NT], m[NT], l[NT];
+  f32x4_t o[NT][kDTiles];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float v[kSteps][8], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const u32x4_t w = raw[nt][k][0];
+      if constexpr (NP == 2) {
+        const u32x4_t w1 = raw[nt][k][1];
+        widen16<float>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
+        widen16<float>(make_uint4(w1[0], w1[1], w1[2], w1[3]), v[k] + 4);
       } else if (a.dtype == CSAHCA_F16) {
-        load16(static_cast<const f16*>(a.q) + at + d, v[k]);
+        widen16<f16>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
       } else {
-        load16(static_cast<const bf16*>(a.q) + at + d, v[k]);
+        widen16<bf16>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
@@ -306,36 +389,24 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
     for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
 
-  int32_t end = part.end;
-  if (!a.ids) {  // the last row of the workgroup sees the most
-    const int32_t last = min((rg + 1) * a.row_waves * NT * 16, a.rows) - 1;
-    end = min(end, (max(len - a.queries + 1 + last / a.group, 0) + kKv8Tile - 1) / kKv8Tile);
-  }
-  const int32_t least = len - a.queries + 1 + row0 / a.group;  // the wavefront's first row sees the least
-  const uint8_t* kbase = a.c.k + (lane % 4) * D + g * 16;
-  const uint8_t* ktail = a.c.k + (lane % 4) * D + kWide * 64 + g * 8;
-  const uint8_t* vbase = a.c.v + n * kKv8Group;
-
-  for (int32_t seg = part.begin; seg < end; seg += kKv8SegTiles) {
-    __syncthreads();
-    subs[threadIdx.x] = kv8_resolve(a, b, h, len, static_cast<int64_t>(seg) * 4 + threadIdx.x);
-    __syncthreads();
+  for (int32_t seg = part.begin; seg < end;) {
     const int32_t seg_end = min(end - seg, kKv8SegTiles);
-    for (int32_t tile = wave % token_waves; tile < seg_end; tile += token_waves) {
-      const Kv8Sub sub = subs[tile * 4 + g];
-      const int64_t koff = static_cast<int64_t>(subs[tile * 4 + n / 4].at) * (kKv8Group * D);
-      const int64_t voff = static_cast<int64_t>(sub.at) * (kKv8Group * D);
-      uint4 kw[4][kWide > 0 ? kWide : 1];
-      uint2 kt[4];
-      uint4 vw[kDTiles];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int w = 0; w < kWide; ++w) kw[t][w] = load_global_u4(kbase + koff + 4 * t * D + 64 * w);
-        if constexpr (kTail) kt[t] = load_global_u2(ktail + koff + 4 * t * D);
+    for (int i = 0; i < kKv8Lookups; ++i) {
+      const int at = i * kKv8Threads + threadIdx.x;
+      if (at < seg_end * 4) sub_scale[at] = make_float2(ks[i], __builtin_amdgcn_logf(fmaxf(vs[i], FLT_MIN)));
+    }
+    lds_barrier();
+
+    // One tile; its successor's K and V are loaded as its own are done with.
+    const auto tile_step = [&](int32_t tile, auto more) {
+      const uint32_t lohi = sub_at[tile * 4 + g].y;
+      const float2 scale = sub_scale[tile * 4 + g];
+      uint32_t next_k = 0u, next_v = 0u;
+      if constexpr (more.value) {
+        next_k = sub_at[(tile + token_waves) * 4 + n / 4].x;
+        next_v = sub_at[(tile + token_waves) * 4 + g].x;
       }
-#pragma unroll
-      for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = load_global_u4(vbase + voff + dt * 16 * kKv8Group);
 
       f32x4_t s[NT][4];
 #pragma unroll
@@ -360,9 +431,11 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
         }
       }
 
-      const int32_t lo = sub.lohi & 0xff, hi = sub.lohi >> 8;
+      if constexpr (more.value) load_k(next_k);
+
+      const int32_t lo = lohi & 0xff, hi = lohi >> 8;
       const int32_t token = (seg + tile) * kKv8Tile + g * kKv8Group;
-      const bool edge = __ballot(sub.lohi != kKv8Whole) != 0 || (!a.ids && (seg + tile + 1) * kKv8Tile > least);
+      const bool edge = __ballot(lohi != kKv8Whole) != 0 || (!a.ids && (seg + tile + 1) * kKv8Tile > least);
       if (edge) {
         // bytes behind the sequence may be NaN, which a weight of 0 does not hide
         uint32_t keep[4];
@@ -381,14 +454,14 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
           vw[dt].w &= keep[3];
         }
       }
-      const float inv_vs = fast_exp2(-sub.lv);
+      const float inv_vs = fast_exp2(-scale.y);
       half8_t pa[NT][NP][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float c = sub.ks * rc[nt];
+        const float c = scale.x * rc[nt];
         float sc[16], top = -__builtin_inff();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = fmaf(s[nt][i / 4][i % 4], c, sub.lv);
+        for (int i = 0; i < 16; ++i) sc[i] = fmaf(s[nt][i / 4][i % 4], c, scale.y);
         if (edge) {
           const int32_t to = a.ids ? hi : min(hi, limit[nt] - token);
 #pragma unroll
@@ -429,6 +502,15 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
             o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pa[nt][p][1], o[nt][dt], 0, 0, 0);
           }
       }
+      if constexpr (more.value) load_v(next_v);
+    };
+    int32_t tile = first;
+    for (; tile + token_waves < seg_end; tile += token_waves) tile_step(tile, std::true_type{});
+    if (tile < seg_end) tile_step(tile, std::false_type{});
+    seg += kKv8SegTiles;
+    if (seg < end) {
+      lds_barrier();  // the segment's entries are done with
+      look_up(seg, min(end - seg, kKv8SegTiles));
     }
   }
 
@@ -469,17 +551,7 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
         const float inv = total != 0.f ? 1.0f / total : 0.f;
         const int64_t at =
             ((static_cast<int64_t>(b) * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D + d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y = acc[e] * inv;
-          if (a.dtype == CSAHCA_F32) {
-            static_cast<float*>(a.out)[at + e] = y;
-          } else if (a.dtype == CSAHCA_F16) {
-            static_cast<f16*>(a.out)[at + e] = from_f32<f16>(y);
-          } else {
-            static_cast<bf16*>(a.out)[at + e] = from_f32<bf16>(y);
-          }
-        }
+        kv8_store4(a, at, acc * inv);
       }
     }
   }
