@@ -19,9 +19,8 @@ constexpr int kKv8MaxPage = 256;     // tokens of a page, at most
 constexpr int kKv8MaxHeadDim = 256;  // a multiple of 32
 constexpr int kKv8LeastExp = -120;   // scales are 2^-120 .. 2^120
 
-// The two formats: the largest magnitude as kTop 2^kTopExp with kTop in
-// [0.5, 1), the decoding of a byte and the encoding of a value that was
-// divided by its scale (round to nearest even; too large: the largest).
+// The two formats: the largest magnitude, and as kTop 2^kTopExp with kTop in
+// [0.5, 1).
 struct E4m3 {
   static constexpr float kMax = 448.0f, kTop = 0.875f;
   static constexpr int kTopExp = 9;
@@ -38,18 +37,6 @@ __device__ __forceinline__ float kv8_decode(uint32_t w) {
     return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(w), Sel);
   } else {
     return static_cast<float>(static_cast<int8_t>(w >> (8 * Sel)));
-  }
-}
-
-// One value to a byte.  NaN is kept as e4m3's NaN; int8 has none and stores 0.
-template <typename F>
-__device__ __forceinline__ uint32_t kv8_encode(float x) {
-  const float c = fminf(fmaxf(x, -F::kMax), F::kMax);
-  if constexpr (std::is_same_v<F, E4m3>) {
-    const float y = x != x ? x : c;
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false)) & 0xffu;
-  } else {
-    return x != x ? 0u : static_cast<uint32_t>(static_cast<int>(rintf(c))) & 0xffu;
   }
 }
 
