@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_join_kernel(const Kv8Attend a
 
 // How a call is laid out over workgroups, from its sizes alone.
 struct Split {
-  int tiles;       // row tiles (16 rows) of a wavefront
+  int tiles;       // row tiles (16 rows) of a wavefront, 1 or 2
   int row_waves;   // wavefronts of a workgroup over the rows, 1, 2 or 4
   int row_groups;
   int min_tiles;   // 64-token tiles of a part, at least (a list: exactly)
@@ -82,13 +82,12 @@ struct Split {
 
 Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t head_dim, int64_t tiles, bool list) {
   Split s;
-  const int most = dtype == CSAHCA_F32 || head_dim > kKv8FourTilesDim ? 2 : 4;
   const int64_t row_tiles = ceil_div(rows, 16);
-  s.tiles = row_tiles <= 1 ? 1 : row_tiles <= 2 ? 2 : most;
+  s.tiles = row_tiles <= 1 || dtype == CSAHCA_F32 || head_dim > kKv8TwoTilesDim ? 1 : 2;
   const int64_t waves = ceil_div(row_tiles, s.tiles);
   s.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
   s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
-  s.target_log2 = s.tiles == 4 ? 8 : 9;  // one workgroup of four row tiles a wavefront fits a CU, else two
+  s.target_log2 = 9;  // two workgroups a CU
   const int round = kKv8Waves / s.row_waves;
   s.min_tiles = round;
   const int64_t target = int64_t{1} << s.target_log2, lanes = kv_heads * s.row_groups;

@@ -19,14 +19,19 @@
 //   * K: 16 bytes of a token's row a load; the order of dimensions in the sum is
 //     free, so a lane's 16 bytes feed two instructions, with q loaded alike.
 //
-// Bytes are exact in f16.  q is: its rows are scaled by a power of two to below
-// 2^15 first (bf16's range is wider than f16's; f32 goes in as two f16, 22
-// bits).  A page's K scale and the row's factor go into the score; its V scale
-// goes into the exponent: p = 2^(s + log2 vs - m) with m the running maximum of
-// that sum, so p V is in units of the largest p vs so far whatever the scales
-// are, and the softmax's sum takes p / vs.  p is rounded to 11 bits (16-bit
-// values) or 22 (f32, two f16), scaled by 2^15: f16 would lose weights below
-// 2^-14 of the largest otherwise.
+// Beside 16-bit values the operands are f16, in which a byte is exact and so is
+// q, its rows scaled by a power of two to below 2^15 (bf16 has the wider range).
+// A page's K scale and the row's factor go into the score; its V scale goes into
+// the exponent: p = 2^(s + log2 vs - m) with m the running maximum of that sum,
+// so p V is in units of the largest p vs so far whatever the scales are, and the
+// softmax's sum takes p / vs (by a third small product, as if V's byte were 1,
+// whose rows keep the sub-blocks apart).  p is rounded to f16's 11 bits.  It is
+// held times 2^11 and m moves only when a score passes it by 4: the sums are
+// rarely rescaled, p stays at most 2^15, and what is lost of a weight for want of
+// exponent is at most 2^-36 of the largest weight.
+//
+// Beside f32 values the operands are bf16, as wide as f32: q and p as three bf16
+// each, 24 bits, of which nothing is lost.
 #pragma once
 
 #include <cfloat>
@@ -40,11 +45,13 @@ constexpr int kKv8Waves = kKv8Threads / kWave;
 constexpr int kKv8Tile = 64;      // tokens a wavefront takes at a time
 constexpr int kKv8SegTiles = 256;  // tiles whose pages a workgroup looks up at once
 constexpr int kKv8Lookups = kKv8SegTiles * 4 / kKv8Threads;  // sub-blocks of a segment a thread
-constexpr int kKv8FourTilesDim = 128;  // head sizes up to which a wavefront holds four row tiles in registers
-constexpr float kKv8PShift = 15.0f;
+constexpr int kKv8TwoTilesDim = 192;  // head sizes up to which a wavefront's registers hold two row tiles
+constexpr float kKv8PShift = 11.0f;  // a weight is held times 2^11 ...
+constexpr float kKv8Slack = 4.0f;    // ... and may pass the running maximum by 2^4
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bhalf8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct Kv8Attend {
@@ -211,26 +218,77 @@ __device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int
   return s;
 }
 
-// Eight bytes as eight f16.
-template <typename F>
-__device__ __forceinline__ half8_t kv8_half8(uint32_t lo, uint32_t hi) {
-  half2_t r[4];
-  if constexpr (std::is_same_v<F, E4m3>) {
-    r[0] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
-    r[1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
-    r[2] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
-    r[3] = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
-  } else {
-    // b + 128 under the exponent of 1024 is the f16 1152 + b; every step is exact
+// The upper halves of two fp32 values: bf16, cut off.
+__device__ __forceinline__ uint32_t kv8_upper_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// Eight bytes as eight f16 (kF32: bf16), which is exact.
+template <typename F, bool kF32>
+__device__ __forceinline__ u32x4_t kv8_operand(uint32_t lo, uint32_t hi) {
+  u32x4_t r;
+  if constexpr (std::is_same_v<F, E4m3> && !kF32) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+  } else if constexpr (std::is_same_v<F, E4m3>) {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  } else if constexpr (!kF32) {
+    // b + 128 under the exponent of 1024 is the f16 1152 + b
     const half2_t off = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
     const uint32_t w[2] = {lo ^ 0x80808080u, hi ^ 0x80808080u};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      r[2 * i] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) - off;
-      r[2 * i + 1] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) - off;
+      r[2 * i] = __builtin_bit_cast(
+          uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04010400u)) - off);
+      r[2 * i + 1] = __builtin_bit_cast(
+          uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, w[i], 0x04030402u)) - off);
+    }
+  } else {
+    const uint32_t w[2] = {lo, hi};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      r[2 * i] = kv8_upper_halves(kv8_decode<Int8, 0>(w[i]), kv8_decode<Int8, 1>(w[i]));
+      r[2 * i + 1] = kv8_upper_halves(kv8_decode<Int8, 2>(w[i]), kv8_decode<Int8, 3>(w[i]));
     }
   }
-  return half8_t{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
+  return r;
+}
+
+template <bool kF32>
+__device__ __forceinline__ f32x4_t kv8_mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+  if constexpr (kF32) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8_t, a), __builtin_bit_cast(bhalf8_t, b), c, 0,
+                                                   0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0,
+                                                  0);
+  }
+}
+
+// Eight fp32 values as operands: one f16 each, or three bf16 that add up to it
+// (the upper 8 bits, those of what is left, and the last ones).
+template <bool kF32, int NP>
+__device__ __forceinline__ void kv8_split(const float (&v)[8], u32x4_t (&out)[NP]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kF32) {
+      float x = v[2 * i], y = v[2 * i + 1];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        out[p][i] = kv8_upper_halves(x, y);
+        x -= __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+        y -= __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+      }
+    } else {
+      const half2_t h = {static_cast<_Float16>(v[2 * i]), static_cast<_Float16>(v[2 * i + 1])};
+      out[0][i] = __builtin_bit_cast(uint32_t, h);
+    }
+  }
 }
 
 // Four values to the output, rounded to its type.
@@ -247,19 +305,26 @@ __device__ __forceinline__ void kv8_store4(const Kv8Attend& a, int64_t at, f32x4
   }
 }
 
-template <int D, typename F, int NP, int NT>
-__global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend a) {
+// Workgroups of a CU: two while a wavefront's registers (K, V, the sums, q, scores
+// and weights) fit 256.
+template <int D, int NP, int NT>
+constexpr int kKv8Blocks = D / 4 * (2 + NT) + NP * NT * D / 8 + 16 * NT + 8 * NP * NT <= 216 ? 2 : 1;
+
+template <int D, typename F, bool kF32, int NT>
+__global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) void kv8_attend_kernel(const Kv8Attend a) {
+  constexpr int NP = kF32 ? 3 : 1;         // operands that make up a value of q or a weight
   constexpr int kSteps = D / 32;           // matrix instructions over D
   constexpr int kWide = D / 64;            // 16-byte loads of a K row
   constexpr bool kTail = D % 64 != 0;      // and one of 8 bytes
   constexpr int kDTiles = D / 16;
   constexpr int kRowPad = D + 4;
   constexpr size_t kMergeBytes = sizeof(float) * kKv8Waves * 16 * kRowPad;
-  constexpr size_t kSubBytes = 16 * kKv8SegTiles * 4;
+  constexpr size_t kSubBytes = 20 * kKv8SegTiles * 4;
   __shared__ __attribute__((aligned(16))) char lds[kMergeBytes > kSubBytes ? kMergeBytes : kSubBytes];
   __shared__ float lds_ml[kKv8Waves][16][2];
   uint2* sub_at = reinterpret_cast<uint2*>(lds);                          // index, valid tokens
   float2* sub_scale = reinterpret_cast<float2*>(lds) + kKv8SegTiles * 4;  // K scale, log2 of the V scale
+  float* sub_inv = reinterpret_cast<float*>(lds) + kKv8SegTiles * 16;     // 1 / V scale
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = lane % 16, g = lane / 16;
@@ -276,7 +341,8 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
   const int32_t heads = a.c.kv_heads * a.group;
 
   // The lane's dimensions of row n of each row tile, as they are stored.
-  u32x4_t raw[NT][kSteps][NP];
+  constexpr int kRaw = kF32 ? 2 : 1;  // 16-byte loads of eight values
+  u32x4_t raw[NT][kSteps][kRaw];
   int32_t limit[NT];  // tokens the row sees
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -288,8 +354,8 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
     for (int k = 0; k < kSteps; ++k) {
       const int d = kTail && k == kSteps - 1 ? kWide * 64 + g * 8 : k / 2 * 64 + g * 16 + k % 2 * 8;
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
-        raw[nt][k][p] = load_global_raw<u32x4_t>(static_cast<const uint8_t*>(a.q) + (at + d) * 2 * NP + 16 * p);
+      for (int p = 0; p < kRaw; ++p)
+        raw[nt][k][p] = load_global_raw<u32x4_t>(static_cast<const uint8_t*>(a.q) + (at + d) * 2 * kRaw + 16 * p);
     }
   }
 
@@ -346,19 +412,22 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
       load_v(sub_at[first * 4 + g].x);
     }
   };
-  look_up(part.begin, min(end - part.begin, kKv8SegTiles));
+  // Before q is converted, where there are registers to hold both.
+  constexpr bool kEarly = NT == 1 && D <= 128;
+  if constexpr (kEarly) look_up(part.begin, min(end - part.begin, kKv8SegTiles));
 
-  // q in f16, its rows scaled to below 2^15
-  half8_t q[NT][NP][kSteps];
+  // q as operands, in f16 its rows scaled to below 2^15
+  u32x4_t q[NT][kSteps][NP];
   float rc[NT], m[NT], l[NT];
   f32x4_t o[NT][kDTiles];
+  const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     float v[kSteps][8], top = 0.f;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
       const u32x4_t w = raw[nt][k][0];
-      if constexpr (NP == 2) {
+      if constexpr (kF32) {
         const u32x4_t w1 = raw[nt][k][1];
         widen16<float>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
         widen16<float>(make_uint4(w1[0], w1[1], w1[2], w1[3]), v[k] + 4);
@@ -367,34 +436,45 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
       } else {
         widen16<bf16>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
     }
-    top = fmaxf(top, xor_lanes(top, 16));
-    top = fmaxf(top, xor_lanes(top, 32));
     int e2 = 15;
-    if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
+    if constexpr (!kF32) {
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = __builtin_ldexpf(v[k][e], 15 - e2);
-        q[nt][0][k][e] = static_cast<_Float16>(y);
-        if constexpr (NP == 2) q[nt][1][k][e] = static_cast<_Float16>(y - static_cast<float>(q[nt][0][k][e]));
-      }
-    rc[nt] = __builtin_ldexpf(a.scale_log2, e2 - 15);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+      top = fmaxf(top, xor_lanes(top, 16));
+      top = fmaxf(top, xor_lanes(top, 32));
+      if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = kF32 ? v[k][e] * sign : __builtin_ldexpf(v[k][e] * sign, 15 - e2);
+      kv8_split<kF32>(v[k], q[nt][k]);
+    }
+    rc[nt] = __builtin_ldexpf(fabsf(a.scale_log2), e2 - 15);
     m[nt] = -FLT_MAX;  // finite: a row of NaN scores still reaches the sums
     l[nt] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
+  // The weights' sums by sub-block: row r < 4 of the product takes those of quarter r.
+  u32x4_t ones;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ones[i] = n != g ? 0u : kF32 ? 0x3f803f80u : 0x3c003c00u;
+  if constexpr (!kEarly) look_up(part.begin, min(end - part.begin, kKv8SegTiles));
 
   for (int32_t seg = part.begin; seg < end;) {
     const int32_t seg_end = min(end - seg, kKv8SegTiles);
 #pragma unroll
     for (int i = 0; i < kKv8Lookups; ++i) {
       const int at = i * kKv8Threads + threadIdx.x;
-      if (at < seg_end * 4) sub_scale[at] = make_float2(ks[i], __builtin_amdgcn_logf(fmaxf(vs[i], FLT_MIN)));
+      if (at < seg_end * 4) {
+        const float lv = __builtin_amdgcn_logf(fmaxf(vs[i], FLT_MIN));
+        sub_scale[at] = make_float2(ks[i], lv);
+        sub_inv[at] = fast_exp2(-lv);
+      }
     }
     lds_barrier();
 
@@ -415,28 +495,35 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
         for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-          half8_t ka;
+          u32x4_t ka;
           if (kTail && k == kSteps - 1) {
-            ka = kv8_half8<F>(kt[t].x, kt[t].y);
+            ka = kv8_operand<F, kF32>(kt[t].x, kt[t].y);
           } else if (k % 2 == 0) {
-            ka = kv8_half8<F>(kw[t][k / 2].x, kw[t][k / 2].y);
+            ka = kv8_operand<F, kF32>(kw[t][k / 2].x, kw[t][k / 2].y);
           } else {
-            ka = kv8_half8<F>(kw[t][k / 2].z, kw[t][k / 2].w);
+            ka = kv8_operand<F, kF32>(kw[t][k / 2].z, kw[t][k / 2].w);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int p = 0; p < NP; ++p)
-              s[nt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[nt][p][k], s[nt][t], 0, 0, 0);
+              s[nt][t] = kv8_mfma<kF32>(ka, q[nt][k][p], s[nt][t]);
         }
       }
 
       if constexpr (more.value) load_k(next_k);
 
       const int32_t lo = lohi & 0xff, hi = lohi >> 8;
-      const int32_t token = (seg + tile) * kKv8Tile + g * kKv8Group;
       const bool edge = __ballot(lohi != kKv8Whole) != 0 || (!a.ids && (seg + tile + 1) * kKv8Tile > least);
       if (edge) {
+        const int32_t token = (seg + tile) * kKv8Tile + g * kKv8Group;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int32_t to = a.ids ? hi : min(hi, limit[nt] - token);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[nt][i / 4][i % 4] = i >= lo && i < to ? s[nt][i / 4][i % 4] : -__builtin_inff();
+        }
         // bytes behind the sequence may be NaN, which a weight of 0 does not hide
         uint32_t keep[4];
 #pragma unroll
@@ -454,52 +541,60 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_attend_kernel(const Kv8Attend
           vw[dt].w &= keep[3];
         }
       }
-      const float inv_vs = fast_exp2(-scale.y);
-      half8_t pa[NT][NP][2];
+
+      // The factor of a lane's scores is not negative, so their maximum is that of
+      // the products (and not 0, so that a masked one stays -inf).
+      float c[NT], top[NT];
+      bool up = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float c = scale.x * rc[nt];
-        float sc[16], top = -__builtin_inff();
+        c[nt] = fmaxf(scale.x * rc[nt], 1e-30f);
+        float most = s[nt][0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[i] = fmaf(s[nt][i / 4][i % 4], c, scale.y);
-        if (edge) {
-          const int32_t to = a.ids ? hi : min(hi, limit[nt] - token);
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[nt][i / 4][i % 4]);
+        most = fmaf(most, c[nt], scale.y);
+        most = fmaxf(most, xor_lanes(most, 16));
+        top[nt] = fmaxf(most, xor_lanes(most, 32));
+        up = up || top[nt] > m[nt] + kKv8Slack;
+      }
+      if (__ballot(up)) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = i >= lo && i < to ? sc[i] : -__builtin_inff();
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[i]);
-        top = fmaxf(top, xor_lanes(top, 16));
-        top = fmaxf(top, xor_lanes(top, 32));
-        top = fmaxf(top, m[nt]);
-        if (__ballot(top > m[nt])) {
-          const float fix = fast_exp2(m[nt] - top);
+        for (int nt = 0; nt < NT; ++nt) {
+          top[nt] = fmaxf(top[nt], m[nt]);
+          const float fix = fast_exp2(m[nt] - top[nt]);
           l[nt] *= fix;
 #pragma unroll
           for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] *= fix;
-          m[nt] = top;
+          m[nt] = top[nt];
         }
-        const float base = m[nt] - kKv8PShift;
-        float sum = 0.f;
+      }
+      const f32x4_t inv_vs = *reinterpret_cast<const f32x4_t*>(sub_inv + tile * 4);
+      u32x4_t pa[NT][2][NP];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = fast_exp2(sc[i] - base);
-          sum += p;
-          pa[nt][0][i / 8][i % 8] = static_cast<_Float16>(p);
-          if constexpr (NP == 2)
-            pa[nt][1][i / 8][i % 8] = static_cast<_Float16>(p - static_cast<float>(pa[nt][0][i / 8][i % 8]));
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base = scale.y - m[nt] + kKv8PShift;
+        f32x4_t sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[nt][2 * half + e / 4][e % 4], c[nt], base));
+          kv8_split<kF32>(p, pa[nt][half]);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) sum = kv8_mfma<kF32>(ones, pa[nt][half][i], sum);
         }
-        l[nt] = fmaf(sum, inv_vs, l[nt]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[nt] = fmaf(sum[i], inv_vs[i], l[nt]);
       }
 #pragma unroll
       for (int dt = 0; dt < kDTiles; ++dt) {
-        const half8_t v0 = kv8_half8<F>(vw[dt].x, vw[dt].y), v1 = kv8_half8<F>(vw[dt].z, vw[dt].w);
+        const u32x4_t v0 = kv8_operand<F, kF32>(vw[dt].x, vw[dt].y), v1 = kv8_operand<F, kF32>(vw[dt].z, vw[dt].w);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pa[nt][p][0], o[nt][dt], 0, 0, 0);
-            o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pa[nt][p][1], o[nt][dt], 0, 0, 0);
+          for (int i = 0; i < NP; ++i) {
+            o[nt][dt] = kv8_mfma<kF32>(v0, pa[nt][0][i], o[nt][dt]);
+            o[nt][dt] = kv8_mfma<kF32>(v1, pa[nt][1][i], o[nt][dt]);
           }
       }
       if constexpr (more.value) load_v(next_v);
@@ -566,13 +661,11 @@ int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
   };
   const auto by_tiles = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    if (a.dtype == CSAHCA_F32) {
-      return tiles == 1 ? go(kv8_attend_kernel<D, F, 2, 1>) : go(kv8_attend_kernel<D, F, 2, 2>);
+    if (a.dtype == CSAHCA_F32) return go(kv8_attend_kernel<D, F, true, 1>);
+    if constexpr (D <= kKv8TwoTilesDim) {
+      if (tiles == 2) return go(kv8_attend_kernel<D, F, false, 2>);
     }
-    if constexpr (D <= kKv8FourTilesDim) {
-      if (tiles == 4) return go(kv8_attend_kernel<D, F, 1, 4>);
-    }
-    return tiles == 1 ? go(kv8_attend_kernel<D, F, 1, 1>) : go(kv8_attend_kernel<D, F, 1, 2>);
+    return go(kv8_attend_kernel<D, F, false, 1>);
   };
   switch (a.c.head_dim / 32) {
     case 1: return by_tiles(std::integral_constant<int, 32>{});

@@ -59,29 +59,36 @@ def same_bytes(got, want):
         assert bad.size == 0, f"{name}: {bad.size} of {x.size} bytes differ, first at {bad[:4]}: {x[bad[:4]]} {y[bad[:4]]}"
 
 
-def bound(want, mass, size, dtype, D, n):
+def bound(want, mass, size, dtype, D, n, peak):
     """Error of one output value, from the roundings on the way to it:
 
     * the result: half a step of its type, which below the least normal value is
       half the least subnormal (f16: 2^-25);
-    * every weight p: one rounding to 11 bits (f16 beside 16-bit values) or to 22
-      (two f16 for f32), and p's own relative error, twice (numerator, sum):
-      the score's |q| |k| products in fp32 (D + 8 roundings; q in 22 bits for
-      f32) times ln 2-free scale, plus 4 roundings of a score of that size and
-      the exponential's two;
+    * every weight p: beside 16-bit values one rounding to f16's 11 bits, and where
+      f16 has no exponent for it half its least step: weights are held times 2^11
+      beside the largest, the step is 2^-24, so 2^-36 of the largest weight a token,
+      n 2^-36 ``peak`` in all; beside f32 24 bits and nothing lost;
+    * p's own relative error, twice (numerator, sum): the score's |q| |k| products
+      in fp32 (D + 8 roundings), 4 roundings of a score of that size and the
+      exponential's two;
     * sums over n tokens in fp32, in pieces of at most 64 terms at a time and
       their rescalings."""
     half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
-    p_bits = 2.0 ** -22 if dtype == F32 else 2.0 ** -11
-    q_bits = 2.0 ** -22 if dtype == F32 else 0.0
-    score = size[..., None] * ((D + 12) * 2.0 ** -24 + q_bits) + 2.0 ** -21
+    p_bits = 2.0 ** -23 if dtype == F32 else 2.0 ** -11
+    lost = 0.0 if dtype == F32 else n * peak * 2.0 ** -36
+    score = size[..., None] * (D + 12) * 2.0 ** -24 + 2.0 ** -21
     sums = (64 + n / 16) * 2.0 ** -24
-    return half * np.abs(want) + mass * (p_bits + 2 * score + 2 * sums) + least
+    return half * np.abs(want) + mass * (p_bits + 2 * score + 2 * sums) + lost + least
 
 
-def close(got, want, mass, size, n):
+def peak_of(cache):
+    return plain.LARGEST[cache[0].dtype] * float(cache[3].max())
+
+
+def close(got, want, mass, size, n, peak):
+    """``peak``: the largest |v| that the scales allow."""
     g = got.double().cpu().numpy()
-    tol = bound(want, mass, size, got.dtype, got.shape[-1], n)
+    tol = bound(want, mass, size, got.dtype, got.shape[-1], n, peak)
     # beyond the type's largest value (f16: from 65520 on) the rounded result is an infinity
     over = np.isinf(torch.from_numpy(want).to(got.dtype).double().numpy())
     bad = np.where(over, g != np.copysign(np.inf, want), ~(np.abs(g - want) <= tol))
@@ -301,7 +308,7 @@ def check_attend(q, cache, dirty, table, lengths, **kw):
     got = native.kv8_decode_forward(q.to(DEV), *to_gpu(dirty), table.to(DEV), lengths.to(DEV), **kw)
     assert got.shape == q.shape and got.dtype == q.dtype
     want, mass, size = plain.attend(q, cache, table, lengths, scale=kw.get("softmax_scale"))
-    close(got, want, mass, size, int(lengths.max()))
+    close(got, want, mass, size, int(lengths.max()), peak_of(cache))
     return got
 
 
@@ -358,7 +365,7 @@ def test_attend_long_context_against_a_device_reference(dtype):
         for h in range(H):
             for g in range(G):
                 want, mass, size = plain._softmax_v(qb[h, g], list(kb[h]), list(vb[h]), D ** -0.5)
-                close(got[b, h * G + g], want, mass, np.float64(size), n)
+                close(got[b, h * G + g], want, mass, np.float64(size), n, peak_of(cache))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
@@ -401,7 +408,7 @@ def test_attend_nan_and_infinite_inputs_stay_in_their_row():
     clean[0, 1], clean[1, 0], clean[2, :, 7] = 0, 0, 0
     assert clean.isfinite().all()
     want, mass, size = plain.attend(q[0:1, 0:1], cache, table[0:1], lengths[0:1])
-    close(got[0:1, 0:1], want, mass, size, 40)
+    close(got[0:1, 0:1], want, mass, size, 40, peak_of(cache))
 
 
 def test_attend_pages_outside_the_pool_are_skipped():
@@ -415,7 +422,7 @@ def test_attend_lengths_outside_the_table():
     lengths = torch.tensor([-5, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
     want, mass, size = plain.attend(q, cache, table, lengths)
     got = native.kv8_decode_forward(q.to(DEV), *to_gpu(cache), table.to(DEV), lengths.to(DEV))
-    close(got, want, mass, size, 48)
+    close(got, want, mass, size, 48, peak_of(cache))
     assert not got[0].any() and not got[2].any()
 
 
@@ -468,7 +475,7 @@ def test_attend_pool_beyond_32_bit_offsets():
 def check_csa(q, cache, dirty, table, lengths, chunks, chunk):
     got = native.kv8_csa_decode_forward(q.to(DEV), *to_gpu(dirty), table.to(DEV), lengths.to(DEV), chunks.to(DEV), chunk)
     want, mass, size = plain.attend(q, cache, table, lengths, chunks=chunks.numpy(), chunk_size=chunk)
-    close(got, want, mass, size, chunks.shape[2] * chunk)
+    close(got, want, mass, size, chunks.shape[2] * chunk, peak_of(cache))
     return got
 
 
