@@ -87,12 +87,13 @@ Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t
   const int64_t waves = ceil_div(row_tiles, s.tiles);
   s.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
   s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
-  s.target_log2 = 9;  // two workgroups a CU
+  s.target_log2 = list || s.row_waves == 4 ? 8 : 10;
   const int round = kKv8Waves / s.row_waves;
-  s.min_tiles = round;
+  // Up to four rounds of a workgroup's wavefronts go undivided, without the join.
+  s.min_tiles = tiles <= 4 * round ? std::max(static_cast<int>(ceil_div(tiles, round)), 1) * round : round;
   const int64_t target = int64_t{1} << s.target_log2, lanes = kv_heads * s.row_groups;
   if (list) {
-    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(tiles * batch * lanes / target + 1, round), round) * round);
+    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(tiles * batch * lanes / target + 1, s.min_tiles), round) * round);
     s.parts = batch * ceil_div(tiles, s.min_tiles);
   } else {
     s.parts = std::min(target / lanes + batch, batch * std::max<int64_t>(ceil_div(tiles, s.min_tiles), 1));
@@ -155,6 +156,8 @@ Kv8Attend args_of(const Kv8Cache& c, const void* q, void* out, int dtype, int64_
   a.queries = static_cast<int32_t>(queries);
   a.group = static_cast<int32_t>(heads / c.kv_heads);
   a.rows = static_cast<int32_t>(queries * a.group);
+  a.page_groups = static_cast<uint32_t>(c.page_size / kKv8Group);
+  a.page_magic = a.page_groups == 1 ? 0u : static_cast<uint32_t>(((uint64_t{1} << 32) + a.page_groups - 1) / a.page_groups);
   a.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
   return a;
 }
@@ -252,7 +255,7 @@ extern "C" int csahca_kv8_csa_decode_forward(const void* q, void* out, int dtype
   if (c.blocks > 0 && top_k > 0) {
     a.ids = chunk_indices;
     a.ids64 = index_dtype == CSAHCA_I64;
-    a.chunk = chunk_size;
+    a.chunk = static_cast<int32_t>(chunk_size);
     a.top_k = static_cast<int32_t>(top_k);
     a.subs = static_cast<int32_t>(subs);
     a.list_tiles = static_cast<int32_t>(tiles);

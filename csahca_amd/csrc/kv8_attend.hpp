@@ -45,6 +45,7 @@ constexpr int kKv8Waves = kKv8Threads / kWave;
 constexpr int kKv8Tile = 64;      // tokens a wavefront takes at a time
 constexpr int kKv8SegTiles = 256;  // tiles whose pages a workgroup looks up at once
 constexpr int kKv8Lookups = kKv8SegTiles * 4 / kKv8Threads;  // sub-blocks of a segment a thread
+constexpr int kKv8GridRows = 32768;   // of a launch: its y dimension, the rest in z
 constexpr int kKv8TwoTilesDim = 192;  // head sizes up to which a wavefront's registers hold two row tiles
 constexpr float kKv8PShift = 11.0f;  // a weight is held times 2^11 ...
 constexpr float kKv8Slack = 4.0f;    // ... and may pass the running maximum by 2^4
@@ -60,7 +61,7 @@ struct Kv8Attend {
   void* out;
   const int32_t* lengths;
   const void* ids;  // listed chunks [batch, kv_heads, top_k]; null: all tokens
-  int64_t chunk;
+  int32_t chunk;
   int32_t ids64;
   int32_t top_k;
   int32_t subs;        // sub-blocks of a chunk, at most
@@ -76,6 +77,8 @@ struct Kv8Attend {
   int32_t min_tiles;   // tiles of a part, at least
   int32_t target_log2; // about 2^target_log2 workgroups over all
   int32_t join_lanes;  // of a joining workgroup, thread groups that share a row's parts
+  uint32_t page_groups;  // groups of 16 tokens of a page, 1 to 16 ...
+  uint32_t page_magic;   // ... and 2^32 / that, rounded up
   float scale_log2;
   float* part_ml;      // [parts, kv_heads, rows, 2]
   float* part_o;       // [parts, kv_heads, rows, D]
@@ -92,11 +95,19 @@ __device__ __forceinline__ int32_t kv8_length(const Kv8Attend& a, int64_t b) {
   return min(max(a.lengths[b], 0), cap);
 }
 
-__device__ __forceinline__ int32_t kv8_wave_sum(int32_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
+// Inclusive prefix sum over the lanes (rows of 16 shifted by 1, 2, 4, 8, then the
+// last lanes of rows and halves passed on).
+__device__ __forceinline__ int32_t kv8_wave_scan(int32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
+
+__device__ __forceinline__ int32_t kv8_wave_sum(int32_t v) { return __builtin_amdgcn_readlane(kv8_wave_scan(v), kWave - 1); }
 
 __device__ __forceinline__ int32_t kv8_tiles(const Kv8Attend& a, int32_t b) {
   return b < a.batch ? (kv8_length(a, b) + kKv8Tile - 1) / kKv8Tile : 0;
@@ -115,19 +126,8 @@ __device__ __forceinline__ int32_t kv8_part_size(const Kv8Attend& a, int32_t* mi
     total += kv8_wave_sum(*mine);
   }
   const int64_t per = (total * a.c.kv_heads * a.row_groups) >> a.target_log2;
-  const int32_t round = kKv8Waves / a.row_waves;
-  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + round - 1) / round * round;
-}
-
-// Inclusive prefix sum over the lanes.
-__device__ __forceinline__ int32_t kv8_wave_scan(int32_t v) {
-  const int lane = threadIdx.x % kWave;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int32_t u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
+  const int32_t round = kKv8Waves / a.row_waves;  // a power of two
+  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + round - 1) & -round;
 }
 
 // The part of index `part` over all sequences, each of which has at least one
@@ -147,11 +147,11 @@ __device__ __forceinline__ Kv8Part kv8_locate(const Kv8Attend& a, int32_t part) 
     const uint64_t hit = __ballot(first + upto > part);
     if (hit) {
       const int at = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      const int32_t n = __shfl(count, at), from = first + __shfl(upto, at) - n;
+      const int32_t n = __builtin_amdgcn_readlane(count, at), from = first + __builtin_amdgcn_readlane(upto, at) - n;
       const int32_t j = part - from;
-      return {base + at, j * size, min((j + 1) * size, __shfl(tiles, at)), n, from};
+      return {base + at, j * size, min((j + 1) * size, __builtin_amdgcn_readlane(tiles, at)), n, from};
     }
-    first += __shfl(upto, kWave - 1);
+    first += __builtin_amdgcn_readlane(upto, kWave - 1);
   }
   return {-1, 0, 0, 0, 0};
 }
@@ -171,7 +171,7 @@ __device__ __forceinline__ void kv8_parts_of(const Kv8Attend& a, int32_t b, int3
     if (a.batch > kWave) tiles = kv8_tiles(a, base + lane);
     const int32_t mine = base + lane <= b ? max((tiles + size - 1) / size, 1) : 0;
     *first += kv8_wave_sum(mine);
-    *count = __shfl(mine, b % kWave);
+    *count = __builtin_amdgcn_readlane(mine, b % kWave);
   }
   *first -= *count;
 }
@@ -185,33 +185,34 @@ struct Kv8Sub {
 };
 constexpr uint32_t kKv8Whole = 16u << 8;
 
-__device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int32_t h, int32_t n, int64_t u) {
+// Sub-block u of sequence b (n tokens) or, with a list, of its chunks.
+__device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int32_t h, int32_t n, uint32_t u) {
   const Kv8Cache& c = a.c;
-  int64_t token = u * kKv8Group;
+  uint32_t group = u;  // of 16 tokens, within the sequence
   int32_t lo = 0, hi = 0;
   if (a.ids) {
-    const int64_t j = static_cast<int32_t>(u) / a.subs;
-    if (j < a.top_k) {
+    const uint32_t j = u / static_cast<uint32_t>(a.subs);
+    if (j < static_cast<uint32_t>(a.top_k)) {
       const int64_t at = (static_cast<int64_t>(b) * c.kv_heads + h) * a.top_k + j;
       const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
-      if (id >= 0 && id <= n / a.chunk) {
-        const int64_t from = id * a.chunk, to = min(from + a.chunk, static_cast<int64_t>(n));
-        token = (from / kKv8Group + (u - j * a.subs)) * kKv8Group;
-        lo = static_cast<int32_t>(max(from - token, static_cast<int64_t>(0)));
-        hi = static_cast<int32_t>(max(min(to - token, static_cast<int64_t>(kKv8Group)), static_cast<int64_t>(0)));
+      if (id >= 0 && id <= static_cast<uint32_t>(n) / static_cast<uint32_t>(a.chunk)) {  // so that its first token is at most n
+        const int32_t from = static_cast<int32_t>(id) * a.chunk, to = from + min(a.chunk, n - from);
+        group = from / kKv8Group + (u - j * a.subs);
+        lo = max(from - static_cast<int32_t>(group) * kKv8Group, 0);
+        hi = max(min(to - static_cast<int32_t>(group) * kKv8Group, kKv8Group), 0);
       }
     }
   } else {
-    hi = static_cast<int32_t>(max(min(n - token, static_cast<int64_t>(kKv8Group)), static_cast<int64_t>(0)));
+    hi = max(min(n - static_cast<int32_t>(u) * kKv8Group, kKv8Group), 0);
   }
   Kv8Sub s{0u, 0u, -1};
   if (hi > lo) {
-    const int32_t block = static_cast<int32_t>(token) / c.page_size;
+    // group / (groups of a page): exact, as group < 2^27 and the divisor is at most 16
+    const uint32_t block = a.page_groups == 1 ? group : __umulhi(group, a.page_magic);
     const int32_t page = kv8_page(c, b, block);
     if (page >= 0) {
-      const int32_t row = static_cast<int32_t>(token) - block * c.page_size;
       s.scale = page * c.kv_heads + h;
-      s.at = static_cast<uint32_t>(s.scale * (c.page_size / kKv8Group) + row / kKv8Group);
+      s.at = static_cast<uint32_t>(s.scale) * a.page_groups + (group - block * a.page_groups);
       s.lohi = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 8;
     }
   }
@@ -221,6 +222,25 @@ __device__ __forceinline__ Kv8Sub kv8_resolve(const Kv8Attend& a, int32_t b, int
 // The upper halves of two fp32 values: bf16, cut off.
 __device__ __forceinline__ uint32_t kv8_upper_halves(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// An address as the compiler cannot see through it (loads from it stay where
+// they are), and a load at a constant offset from one.
+__device__ __forceinline__ uint64_t kv8_opaque(const void* p) {
+  uint64_t a = reinterpret_cast<uint64_t>(p);
+  asm volatile("" : "+v"(a));
+  return a;
+}
+template <typename V>
+__device__ __forceinline__ V kv8_load(uint64_t base, int offset) {
+  return *reinterpret_cast<const __attribute__((address_space(1))) V*>(base + offset);
+}
+
+// The larger of three in one instruction (fmaxf twice also quiets each operand).
+__device__ __forceinline__ float kv8_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 // Eight bytes as eight f16 (kF32: bf16), which is exact.
@@ -328,10 +348,11 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = lane % 16, g = lane / 16;
-  uint32_t x = blockIdx.x;
-  const int32_t h = x % a.c.kv_heads;
-  x /= a.c.kv_heads;
-  const int32_t rg = x % a.row_groups, part_index = x / a.row_groups;
+  // Workgroups in order of heads (which lie next to each other in memory), row
+  // groups and parts.
+  const int32_t h = blockIdx.x, at_part = blockIdx.z * kKv8GridRows + blockIdx.y;
+  const int32_t part_index = a.row_groups == 1 ? at_part : at_part / a.row_groups, rg = at_part - part_index * a.row_groups;
+  if (part_index >= a.parts) return;
   const Kv8Part part = kv8_locate(a, part_index);
   if (part.batch < 0) return;  // fewer parts than the launch allows for
   const int32_t b = part.batch;
@@ -347,8 +368,8 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int32_t r = min(row0 + nt * 16 + n, a.rows - 1);
-    const int32_t qi = r / a.group;
-    const int64_t at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + r % a.group) * D;
+    const int32_t qi = a.queries == 1 ? 0 : r / a.group;
+    const int64_t at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + (r - qi * a.group)) * D;
     limit[nt] = max(len - a.queries + 1 + qi, 0);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
@@ -369,22 +390,23 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
   const uint8_t* ktail = a.c.k + (lane % 4) * D + kWide * 64 + g * 8;
   const uint8_t* vbase = a.c.v + n * kKv8Group;
 
-  uint4 kw[4][kWide > 0 ? kWide : 1];
-  uint2 kt[4];
-  uint4 vw[kDTiles];
+  u32x4_t kw[4][kWide > 0 ? kWide : 1];
+  u32x2_t kt[4];
+  u32x4_t vw[kDTiles];
   const auto load_k = [&](uint32_t at) {
     const int64_t off = static_cast<int64_t>(at) * (kKv8Group * D);
+    const uint64_t wide = kv8_opaque(kbase + off), tail = kv8_opaque(ktail + off);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int w = 0; w < kWide; ++w) kw[t][w] = load_global_u4(kbase + off + 4 * t * D + 64 * w);
-      if constexpr (kTail) kt[t] = load_global_u2(ktail + off + 4 * t * D);
+      for (int w = 0; w < kWide; ++w) kw[t][w] = kv8_load<u32x4_t>(wide, 4 * t * D + 64 * w);
+      if constexpr (kTail) kt[t] = kv8_load<u32x2_t>(tail, 4 * t * D);
     }
   };
   const auto load_v = [&](uint32_t at) {
-    const int64_t off = static_cast<int64_t>(at) * (kKv8Group * D);
+    const uint64_t base = kv8_opaque(vbase + static_cast<int64_t>(at) * (kKv8Group * D));
 #pragma unroll
-    for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = load_global_u4(vbase + off + dt * 16 * kKv8Group);
+    for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = kv8_load<u32x4_t>(base, dt * 16 * kKv8Group);
   };
 
   // The pages of the segment's sub-blocks, then this wavefront's first loads and
@@ -398,7 +420,7 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
       ks[i] = 0.f;
       vs[i] = 1.f;
       if (at < tiles * 4) {
-        const Kv8Sub sub = kv8_resolve(a, b, h, len, static_cast<int64_t>(seg) * 4 + at);
+        const Kv8Sub sub = kv8_resolve(a, b, h, len, static_cast<uint32_t>(seg) * 4 + at);
         sub_at[at] = make_uint2(sub.at, sub.lohi);
         if (sub.scale >= 0) {
           ks[i] = a.c.k_scale[sub.scale];
@@ -490,27 +512,32 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 
       f32x4_t s[NT][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) s[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          u32x4_t ka;
-          if (kTail && k == kSteps - 1) {
-            ka = kv8_operand<F, kF32>(kt[t].x, kt[t].y);
-          } else if (k % 2 == 0) {
-            ka = kv8_operand<F, kF32>(kw[t][k / 2].x, kw[t][k / 2].y);
-          } else {
-            ka = kv8_operand<F, kF32>(kw[t][k / 2].z, kw[t][k / 2].w);
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int t0 = 0; t0 < 4; t0 += 2) {
+          u32x4_t ka[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = t0 + j;
+            if (kTail && k == kSteps - 1) {
+              ka[j] = kv8_operand<F, kF32>(kt[t][0], kt[t][1]);
+            } else if (k % 2 == 0) {
+              ka[j] = kv8_operand<F, kF32>(kw[t][k / 2][0], kw[t][k / 2][1]);
+            } else {
+              ka[j] = kv8_operand<F, kF32>(kw[t][k / 2][2], kw[t][k / 2][3]);
+            }
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-              s[nt][t] = kv8_mfma<kF32>(ka, q[nt][k][p], s[nt][t]);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) s[nt][t0 + j] = kv8_mfma<kF32>(ka[j], q[nt][k][p], s[nt][t0 + j]);
         }
-      }
-
       if constexpr (more.value) load_k(next_k);
 
       const int32_t lo = lohi & 0xff, hi = lohi >> 8;
@@ -534,12 +561,9 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
             if (4 * w + e >= lo && 4 * w + e < hi) keep[w] |= 0xffu << (8 * e);
         }
 #pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt) {
-          vw[dt].x &= keep[0];
-          vw[dt].y &= keep[1];
-          vw[dt].z &= keep[2];
-          vw[dt].w &= keep[3];
-        }
+        for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) vw[dt][w] &= keep[w];
       }
 
       // The factor of a lane's scores is not negative, so their maximum is that of
@@ -549,9 +573,10 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         c[nt] = fmaxf(scale.x * rc[nt], 1e-30f);
-        float most = s[nt][0][0];
+        float most = s[nt][3][3];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) most = fmaxf(most, s[nt][i / 4][i % 4]);
+        for (int i = 0; i < 14; i += 2) most = kv8_max3(most, s[nt][i / 4][i % 4], s[nt][(i + 1) / 4][(i + 1) % 4]);
+        most = fmaxf(most, s[nt][3][2]);
         most = fmaf(most, c[nt], scale.y);
         most = fmaxf(most, xor_lanes(most, 16));
         top[nt] = fmaxf(most, xor_lanes(most, 32));
@@ -587,15 +612,21 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
         for (int i = 0; i < 4; ++i) l[nt] = fmaf(sum[i], inv_vs[i], l[nt]);
       }
 #pragma unroll
-      for (int dt = 0; dt < kDTiles; ++dt) {
-        const u32x4_t v0 = kv8_operand<F, kF32>(vw[dt].x, vw[dt].y), v1 = kv8_operand<F, kF32>(vw[dt].z, vw[dt].w);
+      for (int dt = 0; dt < kDTiles; dt += 2) {
+        u32x4_t va[2][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int j = 0; j < 2; ++j) {
+          va[j][0] = kv8_operand<F, kF32>(vw[dt + j][0], vw[dt + j][1]);
+          va[j][1] = kv8_operand<F, kF32>(vw[dt + j][2], vw[dt + j][3]);
+        }
 #pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            o[nt][dt] = kv8_mfma<kF32>(v0, pa[nt][0][i], o[nt][dt]);
-            o[nt][dt] = kv8_mfma<kF32>(v1, pa[nt][1][i], o[nt][dt]);
-          }
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) o[nt][dt + j] = kv8_mfma<kF32>(va[j][half], pa[nt][half][i], o[nt][dt + j]);
       }
       if constexpr (more.value) load_v(next_v);
     };
@@ -644,8 +675,9 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, total);
       } else {
         const float inv = total != 0.f ? 1.0f / total : 0.f;
+        const int32_t qi = a.queries == 1 ? 0 : r / a.group;
         const int64_t at =
-            ((static_cast<int64_t>(b) * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D + d;
+            ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + (r - qi * a.group)) * D + d;
         kv8_store4(a, at, acc * inv);
       }
     }
@@ -655,7 +687,9 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 // Launch for one format; `tiles` row tiles (16 rows) a wavefront.
 template <typename F>
 int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.parts) * a.row_groups * a.c.kv_heads));
+  const int64_t over = static_cast<int64_t>(a.parts) * a.row_groups;
+  const dim3 grid(static_cast<uint32_t>(a.c.kv_heads), static_cast<uint32_t>(over < kKv8GridRows ? over : kKv8GridRows),
+                  static_cast<uint32_t>(ceil_div(over, kKv8GridRows)));
   const auto go = [&](auto kernel) {
     return launch("kv8_attend_kernel", kernel, grid, dim3(kKv8Threads), 0, stream, a);
   };
