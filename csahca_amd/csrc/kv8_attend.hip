@@ -70,9 +70,10 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_join_kernel(const Kv8Attend a
 
 // How a call is laid out over workgroups, from its sizes alone.
 struct Split {
-  int tiles;       // row tiles (16 rows) of a wavefront, 1 or 2
-  int row_waves;   // wavefronts of a workgroup over the rows, 1, 2 or 4
+  int tiles;       // row tiles (16 rows) of a wavefront, 1 or 2; 0: the kernel of many rows
+  int row_waves;   // wavefronts of a workgroup over the rows, 1, 2, 4 or (many rows) 8
   int row_groups;
+  int round;       // wavefronts over the tokens
   int min_tiles;   // 64-token tiles of a part, at least (a list: exactly)
   int target_log2;
   int64_t parts;   // parts over the batch, at most
@@ -83,12 +84,20 @@ struct Split {
 Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t head_dim, int64_t tiles, bool list) {
   Split s;
   const int64_t row_tiles = ceil_div(rows, 16);
-  s.tiles = row_tiles <= 1 || dtype == CSAHCA_F32 || head_dim > kKv8TwoTilesDim ? 1 : 2;
-  const int64_t waves = ceil_div(row_tiles, s.tiles);
-  s.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
-  s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
-  s.target_log2 = list || s.row_waves == 4 ? 8 : 10;
-  const int round = kKv8Waves / s.row_waves;
+  if (rows > 128 && dtype != CSAHCA_F32) {  // the kernel of many rows, 32 a wavefront
+    s.tiles = 0;
+    s.row_waves = kv8_rows_waves(head_dim);
+    s.row_groups = static_cast<int>(ceil_div(row_tiles, 2 * s.row_waves));
+    s.round = 1;
+  } else {
+    s.tiles = row_tiles <= 1 || dtype == CSAHCA_F32 || head_dim > kKv8TwoTilesDim ? 1 : 2;
+    const int64_t waves = ceil_div(row_tiles, s.tiles);
+    s.row_waves = waves <= 1 ? 1 : waves <= 2 ? 2 : 4;
+    s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
+    s.round = kKv8Waves / s.row_waves;
+  }
+  s.target_log2 = list || s.row_waves >= 4 ? 8 : 10;
+  const int round = s.round;
   // Up to four rounds of a workgroup's wavefronts go undivided, without the join.
   s.min_tiles = tiles <= 4 * round ? std::max(static_cast<int>(ceil_div(tiles, round)), 1) * round : round;
   const int64_t target = int64_t{1} << s.target_log2, lanes = kv_heads * s.row_groups;
@@ -115,6 +124,7 @@ int attend(Kv8Attend a, int format, int64_t tiles, void* workspace, size_t works
     return fail(CSAHCA_ERR_WORKSPACE, "workspace too small for kv8 decode");
   a.row_groups = s.row_groups;
   a.row_waves = s.row_waves;
+  a.round = s.round;
   a.parts = static_cast<int32_t>(s.parts);
   a.min_tiles = s.min_tiles;
   a.target_log2 = s.target_log2;

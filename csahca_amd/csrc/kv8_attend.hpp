@@ -74,6 +74,7 @@ struct Kv8Attend {
   int32_t row_groups;  // workgroups over the rows
   int32_t row_waves;   // wavefronts of a workgroup over the rows; the others split the tokens
   int32_t parts;       // parts of all sequences, at most
+  int32_t round;       // wavefronts over the tokens, a power of two: a part has a multiple of as many tiles
   int32_t min_tiles;   // tiles of a part, at least
   int32_t target_log2; // about 2^target_log2 workgroups over all
   int32_t join_lanes;  // of a joining workgroup, thread groups that share a row's parts
@@ -126,8 +127,7 @@ __device__ __forceinline__ int32_t kv8_part_size(const Kv8Attend& a, int32_t* mi
     total += kv8_wave_sum(*mine);
   }
   const int64_t per = (total * a.c.kv_heads * a.row_groups) >> a.target_log2;
-  const int32_t round = kKv8Waves / a.row_waves;  // a power of two
-  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + round - 1) & -round;
+  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + a.round - 1) & -a.round;
 }
 
 // The part of index `part` over all sequences, each of which has at least one
@@ -684,7 +684,400 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
   }
 }
 
-// Launch for one format; `tiles` row tiles (16 rows) a wavefront.
+// ---------------------------------------------------------------------------
+// Many rows (prompt chunks): 32 rows a wavefront, eight wavefronts a workgroup
+// (four above 128 dimensions).
+//
+// A matrix instruction keeps its SIMD from vector instructions for half its time
+// and those behind it in its wavefront wait with it: beside a 16x16x32 product
+// about two vector instructions are free and each further one costs its time,
+// beside a 32x32x16 (as many operands, twice the work) six are.  So this kernel
+// takes 32x32x16 and sets six vector instructions behind each: the weights of a
+// tile beside the scores of the next, and beside the sums the maximum of the next
+// and the operands of tiles to come.  Those a workgroup's wavefronts make
+// together, each converting its share of a tile's bytes once and passing it on
+// through LDS (two tiles of K and of V, one barrier a tile).  Measured, 2 x 512
+// queries over 16384 tokens, heads 32 / 8 of 128, 271 GFLOP: the kernel above with
+// 32 rows a wavefront 329 us; 32x32x16 and shared operands, phase after phase, 337;
+// interleaved 313; eight wavefronts instead of four 278 (972 TFLOP/s; a library
+// product of 8192^3 in f16 reaches 1250).  What is left: writing operands to LDS
+// 47 us, reading them 20, the loads 22, exponentials 20.
+//
+// Lane l holds row n = l % 32; its half g = l / 32 the tokens of sub-block g of
+// each 32 of a tile: row 8b + 4g + j of a K tile is token 4b + j of sub-block g,
+// so the lane's scores are its sub-block's 16 tokens, and its weights the second
+// product's operand, first 8 and last 8.
+// ---------------------------------------------------------------------------
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16_t kv8_mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// Wavefronts of a workgroup: two a SIMD while a wavefront's registers fit 256.
+constexpr int kv8_rows_waves(int64_t head_dim) { return head_dim <= 128 ? 8 : 4; }
+
+template <int D, typename F>
+__global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_kernel(const Kv8Attend a) {
+  constexpr int kWaves = kv8_rows_waves(D);
+  constexpr int kTiles = kWaves * kWave / 4;  // tiles whose pages are looked up at once: a sub-block a thread
+  constexpr int kSteps = D / 16;   // products over D
+  constexpr int kChunks = D / 32;  // 16-byte loads of a K row by a lane; 32-row tiles of the output
+  constexpr int kPieces = (D / 16 + kWaves - 1) / kWaves;  // of a tile's D / 16 loads of K, those of a wavefront
+  // operands of two tiles, of 64 lanes: load p gives operands 2 p and 2 p + 1
+  __shared__ u32x4_t kops[2][D / 8][kWave], vops[2][D / 8][kWave];
+  __shared__ uint2 sub_at[2][kTiles * 4];      // index, valid tokens
+  __shared__ float4 sub_scale[2][kTiles * 4];  // K scale, log2 of the V scale, 1 / V scale
+  __shared__ uint64_t sub_cut[2][kWaves];          // sub-blocks that are not whole, a bit each
+
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int n = lane % 32, g = lane / 32;
+  const int32_t h = blockIdx.x, at_part = blockIdx.z * kKv8GridRows + blockIdx.y;
+  const int32_t part_index = at_part / a.row_groups, rg = at_part - part_index * a.row_groups;
+  if (part_index >= a.parts) return;
+  const Kv8Part part = kv8_locate(a, part_index);
+  if (part.batch < 0) return;  // fewer parts than the launch allows for
+  const int32_t b = part.batch, len = kv8_length(a, b);
+  const int32_t row0 = (rg * kWaves + wave) * 32;
+  const int32_t heads = a.c.kv_heads * a.group;
+  const int32_t r = min(row0 + n, a.rows - 1), qi = r / a.group;
+  const int64_t q_at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + (r - qi * a.group)) * D;
+  const int32_t limit = max(len - a.queries + 1 + qi, 0);      // tokens the row sees
+  const int32_t least = len - a.queries + 1 + row0 / a.group;  // and the wavefront's first row
+  int32_t end = part.end;
+  if (!a.ids) {  // the workgroup's last row sees the most
+    const int32_t last = min((rg + 1) * kWaves * 32, a.rows) - 1;
+    end = min(end, (max(len - a.queries + 1 + last / a.group, 0) + kKv8Tile - 1) / kKv8Tile);
+  }
+
+  // q in f16, its row scaled to below 2^15: dimension 32 c + 16 g + 8 half + e
+  u32x4_t q[kSteps];
+  float rc;
+  {
+    float v[kSteps][8], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const int64_t at = q_at + k / 2 * 32 + g * 16 + k % 2 * 8;
+      if (a.dtype == CSAHCA_F16) {
+        load16(static_cast<const f16*>(a.q) + at, v[k]);
+      } else {
+        load16(static_cast<const bf16*>(a.q) + at, v[k]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+    }
+    top = fmaxf(top, xor_lanes(top, 32));
+    int e2 = 15;
+    if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
+    const float sign = a.scale_log2 < 0.f ? -1.f : 1.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = __builtin_ldexpf(v[k][e] * sign, 15 - e2);
+      u32x4_t one[1];
+      kv8_split<false>(v[k], one);
+      q[k] = one[0];
+    }
+    rc = __builtin_ldexpf(fabsf(a.scale_log2), e2 - 15);
+  }
+  float m = -FLT_MAX, l = 0.f;
+  f32x16_t o[kChunks];
+#pragma unroll
+  for (int dt = 0; dt < kChunks; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+
+  // Sub-blocks of 64 tiles from tile `seg` on, into buffer `buf`.
+  const auto look_up = [&](int32_t seg, int buf) {
+    const Kv8Sub sub = kv8_resolve(a, b, h, len, static_cast<uint32_t>(seg) * 4 + threadIdx.x);
+    sub_at[buf][threadIdx.x] = make_uint2(sub.at, sub.lohi);
+    const uint64_t cut = __ballot(sub.lohi != kKv8Whole);
+    if (lane == 0) sub_cut[buf][wave] = cut;
+    float ks = 0.f, vs = 1.f;
+    if (sub.scale >= 0) {
+      ks = a.c.k_scale[sub.scale];
+      vs = a.c.v_scale[sub.scale];
+    }
+    const float lv = __builtin_amdgcn_logf(fmaxf(vs, FLT_MIN));
+    sub_scale[buf][threadIdx.x] = make_float4(ks, lv, fast_exp2(-lv), 0.f);
+  };
+  // Entry of a tile's sub-block s (tiles are counted from the part's first).
+  const auto entry = [](int32_t tile, int s) { return tile % kTiles * 4 + s; };
+
+  // This wavefront's loads of a tile's K and of its V (behind the last one it
+  // repeats that), and their operands into LDS.
+  u32x4_t kpiece[kPieces], vpiece[kPieces];
+  const auto piece_of = [&](int i) { return min(wave + kWaves * i, D / 16 - 1); };
+  const auto k_at = [&](int32_t tile, int i) {
+    return sub_at[tile / kTiles % 2][entry(tile, 2 * (piece_of(i) / kChunks) + n / 4 % 2)].x;
+  };
+  const auto v_at = [&](int32_t tile, int i) {
+    return sub_at[tile / kTiles % 2][entry(tile, 2 * (piece_of(i) / kChunks) + g)].x;
+  };
+  const uint8_t* kbase = a.c.k + (n / 8 * 4 + n % 4) * D + g * 16;
+  const uint8_t* vbase = a.c.v + n * kKv8Group;
+  const auto fetch_k = [&](int i, uint32_t at) {
+    kpiece[i] = load_global_raw<u32x4_t>(kbase + (static_cast<int64_t>(at) * (kKv8Group * D) + piece_of(i) % kChunks * 32));
+  };
+  const auto fetch_v = [&](int i, uint32_t at) {
+    vpiece[i] = load_global_raw<u32x4_t>(
+        vbase + (static_cast<int64_t>(at) * (kKv8Group * D) + piece_of(i) % kChunks * 32 * kKv8Group));
+  };
+  const auto pass_k = [&](int32_t tile, int i, int half) {
+    kops[tile % 2][2 * piece_of(i) + half][lane] = kv8_operand<F, false>(kpiece[i][2 * half], kpiece[i][2 * half + 1]);
+  };
+  const auto pass_v = [&](int32_t tile, int i, int half) {
+    vops[tile % 2][2 * piece_of(i) + half][lane] = kv8_operand<F, false>(vpiece[i][2 * half], vpiece[i][2 * half + 1]);
+  };
+  // Masks a tile's scores, and its bytes of V on the way to LDS: those behind the
+  // sequence may be NaN, which a weight of 0 does not hide.
+  const auto cut_of = [&](int32_t tile) {
+    return reinterpret_cast<const uint8_t*>(sub_cut[tile / kTiles % 2])[tile % kTiles / 2] >> (tile % 2 * 4) & 15;
+  };
+  const auto mask = [&](int32_t tile, uint32_t cut, f32x16_t (&s)[2]) {
+    if (__builtin_amdgcn_readfirstlane(cut) != 0 || (!a.ids && (part.begin + tile + 1) * kKv8Tile > least)) {
+      uint32_t lohi[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) lohi[u] = sub_at[tile / kTiles % 2][entry(tile, 2 * u + g)].y;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int32_t lo = lohi[u] & 0xff, hi = lohi[u] >> 8;
+        const int32_t to = a.ids ? hi : min(hi, limit - ((part.begin + tile) * kKv8Tile + (2 * u + g) * kKv8Group));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = i >= lo && i < to ? s[u][i] : -__builtin_inff();
+      }
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        const uint32_t own = piece_of(i) / kChunks ? lohi[1] : lohi[0];
+        const int32_t lo = own & 0xff, hi = own >> 8;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t keep = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * k + e >= lo && 4 * k + e < hi) keep |= 0xffu << (8 * e);
+          vpiece[i][k] &= keep;
+        }
+      }
+    }
+  };
+  const auto scores = [&](int32_t tile, f32x16_t (&s)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[u] = kv8_mfma32(kops[tile % 2][u * kSteps + k][lane], q[k], s[u]);
+  };
+
+  // Of a tile: the factor of a lane's scores, log2 of the V scale and 1 / that.
+  struct Scale {
+    float c[2], lv[2], inv[2];
+  };
+  const auto scale_of = [&](int32_t tile) {
+    Scale x;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float4 e = sub_scale[tile / kTiles % 2][entry(tile, 2 * u + g)];
+      x.c[u] = fmaxf(e.x * rc, 1e-30f);  // not 0, so that a masked score stays -inf
+      x.lv[u] = e.y;
+      x.inv[u] = e.z;
+    }
+    return x;
+  };
+  const auto top_of = [&](const Scale& x, const float (&most)[2]) {
+    const float top = fmaxf(fmaf(most[0], x.c[0], x.lv[0]), fmaf(most[1], x.c[1], x.lv[1]));
+    return fmaxf(top, xor_lanes(top, 32));
+  };
+
+  // Tile `tile`, whose scores are in `s`, and the next one's scores into `t`.  A
+  // product waits for the one before it and everything behind it waits with it,
+  // so each is followed by the vector instructions that it hides.
+  const int32_t tiles = end - part.begin;
+  Scale now;
+  float top = 0.f;  // of the tile's scores
+  const auto step = [&](int32_t tile, f32x16_t (&s)[2], f32x16_t (&t)[2]) {
+    if (tile % kTiles == 0 && tile + kTiles < tiles)
+      look_up(part.begin + tile + kTiles, tile / kTiles % 2 ^ 1);
+    const int32_t next = min(tile + 1, tiles - 1);
+    const uint32_t cut = cut_of(next);
+    constexpr int kAhead = 3;  // operands read ahead of their product
+    const u32x4_t(*kop)[kWave] = kops[(tile + 1) % 2];
+    const u32x4_t(*vop)[kWave] = vops[tile % 2];
+    u32x4_t ready[kAhead];
+    const auto k_operand = [&](int i) { return kop[i % 2 * kSteps + i / 2][lane]; };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ready[i] = k_operand(i);
+    if (__ballot(top > m + kKv8Slack)) {
+      top = fmaxf(top, m);
+      const float fix = fast_exp2(m - top);
+      l *= fix;
+#pragma unroll
+      for (int dt = 0; dt < kChunks; ++dt) o[dt] *= fix;
+      m = top;
+    }
+
+    // the weights, beside the next tile's scores
+    u32x4_t pa[2][2];
+    const float base[2] = {now.lv[0] - m + kKv8PShift, now.lv[1] - m + kKv8PShift};
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[u][i] = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps; ++i) {
+      t[i % 2] = kv8_mfma32(ready[i % kAhead], q[i / 2], t[i % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < 2 * kSteps) {
+        ready[i % kAhead] = k_operand(i + kAhead);
+      } else {
+        ready[i % kAhead] = vop[i + kAhead - 2 * kSteps][lane];
+      }
+#pragma unroll
+      for (int w = i * 8 / kSteps; w < (i + 1) * 8 / kSteps; ++w) {  // its share of the 16 pairs of scores
+        const int v = w / 8, e = w % 8;
+        const half2_t p = {static_cast<_Float16>(fast_exp2(fmaf(s[v][2 * e], now.c[v], base[v]))),
+                           static_cast<_Float16>(fast_exp2(fmaf(s[v][2 * e + 1], now.c[v], base[v])))};
+        sum[v] = __builtin_amdgcn_fdot2(p, half2_t{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, sum[v], false);
+        uint32_t bits = __builtin_bit_cast(uint32_t, p);
+        asm volatile("" : "+v"(bits), "+v"(sum[v]));  // here, not behind the next branch
+        pa[v][e / 4][e % 4] = bits;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    l = fmaf(sum[0], now.inv[0], fmaf(sum[1], now.inv[1], l));
+    mask(next, cut, t);
+
+    // the sums, beside the operands and the loads of tiles to come and the next maximum
+    constexpr int kProducts = 4 * kChunks, kOperands = 4 * kPieces;
+    float most[2] = {t[0][15], t[1][15]};
+    uint32_t at = 0;  // where the next load begins
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {  // operand i: 32 tokens u, dimensions dt, tokens 8 half .. of each lane
+      const int u = i / (2 * kChunks), dt = i / 2 % kChunks, half = i % 2;
+      o[dt] = kv8_mfma32(ready[(2 * kSteps + i) % kAhead], pa[u][half], o[dt]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < kProducts) ready[(2 * kSteps + i) % kAhead] = vop[i + kAhead][lane];
+      if (i == 0) {
+        now = scale_of(next);
+        at = v_at(min(tile + 2, tiles - 1), 0);
+      }
+      // its share of the 16 maxima, and of the operands: V of tile + 1, then K of
+      // tile + 2, in the buffer of this one; behind a load's second operand the next load
+#pragma unroll
+      for (int w = i * 16 / kProducts; w < (i + 1) * 16 / kProducts; ++w)
+        most[w / 8] = w % 8 < 7 ? kv8_max3(most[w / 8], t[w / 8][w % 8 * 2], t[w / 8][w % 8 * 2 + 1])
+                                : fmaxf(most[w / 8], t[w / 8][14]);
+#pragma unroll
+      for (int w = i * kOperands / kProducts; w < (i + 1) * kOperands / kProducts; ++w) {
+        if (w < kOperands / 2) {
+          pass_v(tile + 1, w / 2, w % 2);
+          if (w % 2) {
+            fetch_v(w / 2, at);
+            at = w / 2 + 1 < kPieces ? v_at(min(tile + 2, tiles - 1), w / 2 + 1) : k_at(min(tile + 3, tiles - 1), 0);
+          }
+        } else {
+          pass_k(tile, w / 2 - kPieces, w % 2);
+          if (w % 2) {
+            fetch_k(w / 2 - kPieces, at);
+            if (w + 1 < kOperands) at = k_at(min(tile + 3, tiles - 1), w / 2 - kPieces + 1);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    top = top_of(now, most);
+    lds_barrier();
+  };
+
+  if (tiles > 0) {
+    f32x16_t s0[2], s1[2];
+    look_up(part.begin, 0);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      fetch_k(i, k_at(0, i));
+      fetch_v(i, v_at(0, i));
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kPieces; ++i) pass_k(0, i / 2, i % 2);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) fetch_k(i, k_at(min(1, tiles - 1), i));
+    lds_barrier();
+    scores(0, s0);
+    mask(0, cut_of(0), s0);
+    now = scale_of(0);
+    float most[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      most[u] = s0[u][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) most[u] = fmaxf(most[u], s0[u][i]);
+    }
+    top = top_of(now, most);
+#pragma unroll
+    for (int i = 0; i < 2 * kPieces; ++i) {
+      pass_v(0, i / 2, i % 2);
+      pass_k(1, i / 2, i % 2);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      fetch_v(i, v_at(min(1, tiles - 1), i));
+      fetch_k(i, k_at(min(2, tiles - 1), i));
+    }
+    lds_barrier();
+    if (row0 < a.rows) {
+      for (int32_t tile = 0; tile < tiles; tile += 2) {
+        step(tile, s0, s1);
+        if (tile + 1 < tiles) step(tile + 1, s1, s0);
+      }
+    } else {  // no rows: the operands alone
+      for (int32_t tile = 0; tile < tiles; ++tile) {
+        if (tile % kTiles == 0 && tile + kTiles < tiles) look_up(part.begin + tile + kTiles, tile / kTiles % 2 ^ 1);
+        mask(min(tile + 1, tiles - 1), cut_of(min(tile + 1, tiles - 1)), s0);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          pass_v(tile + 1, i, 0);
+          pass_v(tile + 1, i, 1);
+          fetch_v(i, v_at(min(tile + 2, tiles - 1), i));
+          pass_k(tile, i, 0);
+          pass_k(tile, i, 1);
+          fetch_k(i, k_at(min(tile + 3, tiles - 1), i));
+        }
+        lds_barrier();
+      }
+    }
+  }
+
+  l += xor_lanes(l, 32);
+  if (row0 + n >= a.rows) return;
+  if (part.count > 1) {
+    const int64_t slot = (static_cast<int64_t>(part_index) * a.c.kv_heads + h) * a.rows + r;
+#pragma unroll
+    for (int dt = 0; dt < kChunks; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4_t*>(a.part_o + slot * D + dt * 32 + 8 * i + 4 * g) =
+            f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(m, l);
+  } else {
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int dt = 0; dt < kChunks; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        kv8_store4(a, q_at + dt * 32 + 8 * i + 4 * g,
+                   f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]} * inv);
+  }
+}
+
+// Launch for one format; `tiles` row tiles (16 rows) a wavefront, 0: the kernel of
+// many rows.
 template <typename F>
 int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
   const int64_t over = static_cast<int64_t>(a.parts) * a.row_groups;
@@ -696,6 +1089,9 @@ int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
   const auto by_tiles = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
     if (a.dtype == CSAHCA_F32) return go(kv8_attend_kernel<D, F, true, 1>);
+    if (tiles == 0)
+      return launch("kv8_attend_rows_kernel", kv8_attend_rows_kernel<D, F>, grid, dim3(kv8_rows_waves(D) * kWave), 0, stream,
+                    a);
     if constexpr (D <= kKv8TwoTilesDim) {
       if (tiles == 2) return go(kv8_attend_kernel<D, F, false, 2>);
     }

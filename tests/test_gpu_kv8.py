@@ -492,6 +492,43 @@ def test_csa_chunk_sizes(chunk, top_k, fmt, dtype, page):
     check_csa(q, cache, dirty, table, lengths, chunks, chunk)
 
 
+@pytest.mark.parametrize("G", [17, 40, 100])
+@pytest.mark.parametrize("fmt,dtype", [(E4M3, BF16), (INT8, F16), (E4M3, F32)])
+def test_csa_many_heads_share_a_list(G, fmt, dtype):
+    q, cache, dirty, table, lengths = attend_case(2, 1, 1, G, 96, 48, (301, 77), fmt, dtype, seed=G, stale=0x7f)
+    chunks = torch.tensor([[[3, 0, -1, 9, 4, 4]], [[1, 0, 2, 3, 0, 7]]], dtype=torch.int32)
+    check_csa(q, cache, dirty, table, lengths, chunks, 36)
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 160, 192, 224, 256])
+@pytest.mark.parametrize("fmt,dtype", [(E4M3, BF16), (INT8, F16)])
+def test_attend_many_rows_of_every_head_size(D, fmt, dtype):
+    """More rows than a workgroup of the kernel for many takes, a few of the last one."""
+    check_attend(*attend_case(3, 45, 1, 3, D, 32, (0, 44, 130), fmt, dtype, seed=D + 1, stale=0x7f))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_attend_many_rows_over_many_tiles(dtype):
+    """A prompt chunk over thousands of tokens: several lookups of pages, several
+    parts, against fp64 on the device."""
+    B, Q, H, G, D, page = 2, 70, 1, 2, 64, 64
+    lens = (9000, 4161)
+    blocks = -(-max(lens) // page)
+    cache = to_gpu(filled(B * blocks, H, page, D, E4M3, seed=1, spread=1))
+    table = table_of(B, blocks, B * blocks, seed=2).to(DEV)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = torch.randn(B, Q, H * G, D, generator=gen(3)).to(dtype).to(DEV)
+    got = native.kv8_decode_forward(q, *cache, table, lengths)
+    k, v = native.kv8_read(*cache, table, lengths, max(lens), dtype=F32)
+    for b in range(B):
+        for i in (0, 1, 37, Q - 1):
+            n = lens[b] - Q + 1 + i
+            kb, vb, qb = (t.double().cpu().numpy() for t in (k[b, 0, :n], v[b, 0, :n], q[b, i]))
+            for h in range(G):
+                want, mass, size = plain._softmax_v(qb[h], list(kb), list(vb), D ** -0.5)
+                close(got[b, i, h], want, mass, np.float64(size), n, peak_of(cache))
+
+
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
 def test_csa_ids_that_are_negative_repeated_or_too_large(index):
     B, H, G, D, page, chunk = 6, 1, 3, 64, 16, 24

@@ -103,7 +103,7 @@ def test_workspace_sizes(lib):
     # parts of at least 4 tiles of 64 tokens: 32 for 8192 tokens, each a row of 128 values, a maximum and a sum
     assert f(2, 1, 1, 8, 8, 128, 64, 128) == 32 * 8 * 130 * 4
     assert f(2, big, big, big, 1, 128, 64, big) == 0 and g(2, big, big, 1, 128, big, big) == 0
-    assert f(0, 4, 50, 64, 8, 256, 256, 4096) > 0 and g(2, 32, 8, 8, 128, 32, 64) > 0
+    assert f(0, 4, 50, 64, 8, 256, 256, 4096) > 0 and g(2, 1, 8, 8, 128, 64, 64) > 0
 
 
 def test_missing_workspace_is_reported(lib):
