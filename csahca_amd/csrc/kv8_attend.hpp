@@ -243,6 +243,9 @@ __device__ __forceinline__ float kv8_max3(float a, float b, float c) {
   return r;
 }
 
+// 0x80 in each byte that is an e4m3 NaN.
+__device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Eight bytes as eight f16 (kF32: bf16), which is exact.
 template <typename F, bool kF32>
 __device__ __forceinline__ u32x4_t kv8_operand(uint32_t lo, uint32_t hi) {
@@ -564,6 +567,46 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
         for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
           for (int w = 0; w < 4; ++w) vw[dt][w] &= keep[w];
+        if (std::is_same_v<F, E4m3> && !a.ids && a.queries > 1) {
+          // A token that later queries see may hold NaN too: it is taken out, and the
+          // sums of the rows that do see it are made NaN by a product of ones.
+          uint32_t any = 0;
+#pragma unroll
+          for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) any |= kv8_nan_bytes(vw[dt][w]);
+          if (__ballot(any != 0)) {
+            u32x4_t seen[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int32_t to = min(hi, limit[nt] - token);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t one = kF32 ? 0x3f80u : 0x3c00u;
+                seen[nt][i / 4][i % 4] = (2 * i >= lo && 2 * i < to ? one : 0u) |
+                                         (2 * i + 1 >= lo && 2 * i + 1 < to ? one << 16 : 0u);
+              }
+            }
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt) {
+              uint32_t nan[4];
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                nan[w] = kv8_nan_bytes(vw[dt][w]) >> 7;
+                vw[dt][w] &= ~(nan[w] * 0xffu);
+                nan[w] *= 0x38u;  // 1.0
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                f32x4_t hit{0.f, 0.f, 0.f, 0.f};
+                hit = kv8_mfma<kF32>(kv8_operand<F, kF32>(nan[0], nan[1]), seen[nt][0], hit);
+                hit = kv8_mfma<kF32>(kv8_operand<F, kF32>(nan[2], nan[3]), seen[nt][1], hit);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nt][dt][i] = hit[i] > 0.f ? __builtin_nanf("") : o[nt][dt][i];
+              }
+            }
+          }
+        }
       }
 
       // The factor of a lane's scores is not negative, so their maximum is that of
@@ -729,6 +772,8 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
   __shared__ uint2 sub_at[2][kTiles * 4];      // index, valid tokens
   __shared__ float4 sub_scale[2][kTiles * 4];  // K scale, log2 of the V scale, 1 / V scale
   __shared__ uint64_t sub_cut[2][kWaves];          // sub-blocks that are not whole, a bit each
+  __shared__ uint16_t nans[2][D][4];               // tokens of a sub-block whose V is NaN ...
+  __shared__ uint32_t nan_at[2][kWaves];           // ... and whether a wavefront found any
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = lane % 32, g = lane / 32;
@@ -744,6 +789,9 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
   const int64_t q_at = ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + (r - qi * a.group)) * D;
   const int32_t limit = max(len - a.queries + 1 + qi, 0);      // tokens the row sees
   const int32_t least = len - a.queries + 1 + row0 / a.group;  // and the wavefront's first row
+  // The first row of all waves sees the tokens before this tile.
+  const int32_t all_see =
+      a.ids ? INT32_MAX : max(len - a.queries + 1 + rg * kWaves * 32 / a.group, 0) / kKv8Tile - part.begin;
   int32_t end = part.end;
   if (!a.ids) {  // the workgroup's last row sees the most
     const int32_t last = min((rg + 1) * kWaves * 32, a.rows) - 1;
@@ -860,6 +908,39 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
         }
       }
     }
+    if (std::is_same_v<F, E4m3> && tile >= all_see) {
+      // A token that later queries see may hold NaN too: it is taken out and noted.
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t nan = kv8_nan_bytes(vpiece[i][k]) >> 7;
+          vpiece[i][k] &= ~(nan * 0xffu);
+          bits |= ((nan * 0x10204080u) >> 28) << (4 * k);  // the four bytes' bits together
+        }
+        nans[tile % 2][piece_of(i) % kChunks * 32 + n][2 * (piece_of(i) / kChunks) + g] = static_cast<uint16_t>(bits);
+        any |= bits;
+      }
+      const bool found = __ballot(any != 0) != 0;
+      if (lane == 0) nan_at[tile % 2][wave] = found;
+    }
+  };
+  // The sums of the rows that see a token whose V is NaN become NaN.
+  const auto spread_nans = [&](int32_t tile) {
+    uint32_t any = 0;
+    for (int w = 0; w < kWaves; ++w) any |= nan_at[tile % 2][w];
+    if (__builtin_amdgcn_readfirstlane(any) == 0) return;
+    const int32_t sees = limit - (part.begin + tile) * kKv8Tile;
+    const uint64_t seen = sees >= kKv8Tile ? ~uint64_t{0} : sees <= 0 ? 0u : (uint64_t{1} << sees) - 1;
+#pragma unroll
+    for (int dt = 0; dt < kChunks; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint64_t has = *reinterpret_cast<const uint64_t*>(nans[tile % 2][dt * 32 + i / 4 * 8 + 4 * g + i % 4]);
+        if (has & seen) o[dt][i] = __builtin_nanf("");
+      }
   };
   const auto scores = [&](int32_t tile, f32x16_t (&s)[2]) {
 #pragma unroll
@@ -992,6 +1073,7 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
       __builtin_amdgcn_sched_barrier(0);
     }
     top = top_of(now, most);
+    if (std::is_same_v<F, E4m3> && tile >= all_see) spread_nans(tile);
     lds_barrier();
   };
 

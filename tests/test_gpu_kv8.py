@@ -411,6 +411,28 @@ def test_attend_nan_and_infinite_inputs_stay_in_their_row():
     close(got[0:1, 0:1], want, mass, size, 40, peak_of(cache))
 
 
+@pytest.mark.parametrize("Q,G,D", [(3, 2, 64), (20, 1, 96), (70, 1, 64), (70, 3, 128), (90, 4, 192), (150, 2, 32)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attend_nan_in_a_later_query_s_token_stays_with_its_seers(Q, G, D, dtype):
+    """V of a token that only the later queries of the call see is NaN (and K of
+    another): the earlier queries are as if it were not there."""
+    n = Q + 40
+    q, cache, _, table, lengths = attend_case(2, Q, 1, G, D, 16, (n, n), E4M3, dtype, seed=Q)
+    vb, kb = cache.v_cache.view(torch.uint8), cache.k_cache.view(torch.uint8)
+    at_v, at_k = n - Q // 2, n - 1  # seen from query Q - Q // 2 on, and by the last
+    vb[int(table[0, at_v // 16]), 0, 0, 5, at_v % 16] = 0xff
+    vb[int(table[0, at_v // 16]), 0, 0, D - 1, at_v % 16] = 0x7f
+    kb[int(table[1, at_k // 16]), 0, at_k % 16, 3] = 0x7f
+    got = native.kv8_decode_forward(q.to(DEV), *to_gpu(cache), table.to(DEV), lengths.to(DEV))
+    want, mass, size = plain.attend(q, cache, table, lengths)
+    first = at_v - (n - Q)
+    assert np.isnan(want[0, first:, :, 5]).all() and np.isnan(want[1, -1]).all() and np.isfinite(want[0, :first]).all()
+    assert np.array_equal(np.isnan(got.float().cpu().numpy()), np.isnan(want))
+    fine = torch.from_numpy(np.isnan(want))
+    got, want, mass = got.cpu().masked_fill(fine, 0), np.nan_to_num(want), np.nan_to_num(mass)
+    close(got, want, mass, np.nan_to_num(size), n, peak_of(cache))
+
+
 def test_attend_pages_outside_the_pool_are_skipped():
     q, cache, _, table, lengths = attend_case(3, 1, 2, 1, 64, 16, (60, 60, 30), INT8, F16, seed=7)
     table[0, 1], table[1, 0], table[1, 1], table[1, 2], table[1, 3] = -7, -1, 10 ** 6, -2 ** 31, 2 ** 31 - 1
