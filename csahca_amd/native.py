@@ -1117,54 +1117,55 @@ _KV8_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _KV8_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
-def _kv8_cache_error(k_cache, v_cache, k_scale, v_scale, block_table):
-    if not (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda and block_table.is_cuda):
-        return "the cache, its scales and block_table must be CUDA tensors"
-    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
-        return "k_cache and v_cache must be contiguous"
-    if k_cache.dim() != 4:
-        return "k_cache must be [num_pages, kv_heads, page_size, head_dim]"
-    if k_cache.dtype not in _KV8_FORMATS:
-        return "k_cache must be float8_e4m3fn or int8"
+def _kv8_cache(dev, k_cache, v_cache, k_scale, v_scale, block_table):
+    """Checks a cache and its block table (on device ``dev``); returns its part of
+    the library's arguments (pointers, format, pages, page size, the table with
+    its columns and row stride) and the cache's heads and head_dim.  Inline tests
+    on values read once: they run on every eager call."""
+    shape, table, fmt = k_cache.shape, block_table.shape, _KV8_FORMATS.get(k_cache.dtype)
+    if dev < 0 or not (k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device()
+                       == block_table.get_device() == dev):
+        _kv8_refuse_devices(dev, k_cache, v_cache, k_scale, v_scale, block_table)
+    if len(shape) != 4:
+        raise RuntimeError("k_cache must be [num_pages, kv_heads, page_size, head_dim]")
+    P, H, page, D = shape
+    if fmt is None:
+        raise RuntimeError("k_cache must be float8_e4m3fn or int8")
     if v_cache.dtype != k_cache.dtype:
-        return "k_cache and v_cache dtype must match"
-    P, H, page, D = k_cache.shape
+        raise RuntimeError("k_cache and v_cache dtype must match")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise RuntimeError("k_cache and v_cache must be contiguous")
     if page <= 0 or page > 256 or page % 16:
-        return "page_size must be a multiple of 16, at most 256"
+        raise RuntimeError("page_size must be a multiple of 16, at most 256")
     if D <= 0 or D > 256 or D % 32:
-        return "head_dim must be a multiple of 32, at most 256"
-    if tuple(v_cache.shape) != (P, H, page // 16, D, 16):
-        return "v_cache must be [num_pages, kv_heads, page_size / 16, head_dim, 16]"
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or tuple(s.shape) != (P, H) or not s.is_contiguous():
-            return "scales must be contiguous float32 [num_pages, kv_heads]"
-    if block_table.dim() != 2 or block_table.dtype != torch.int32:
-        return "block_table must be int32 [batch, blocks]"
-    if block_table.shape[1] > 1 and block_table.stride(1) != 1:
-        return "block_table rows must be contiguous"
-    return None
+        raise RuntimeError("head_dim must be a multiple of 32, at most 256")
+    if v_cache.shape != (P, H, page // 16, D, 16):
+        raise RuntimeError("v_cache must be [num_pages, kv_heads, page_size / 16, head_dim, 16]")
+    if not (k_scale.dtype is v_scale.dtype is torch.float32 and k_scale.shape == v_scale.shape == (P, H)
+            and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        raise RuntimeError("scales must be contiguous float32 [num_pages, kv_heads]")
+    if len(table) != 2 or block_table.dtype is not torch.int32:
+        raise RuntimeError("block_table must be int32 [batch, blocks]")
+    rows, blocks = table
+    stride, step = block_table.stride()
+    if blocks > 1 and step != 1:
+        raise RuntimeError("block_table rows must be contiguous")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), fmt, P, page,
+            block_table.data_ptr(), blocks, stride if rows > 1 else blocks), H, D
 
 
-def _kv8_lengths_error(name, t, batch, optional=False):
-    """Of an int32 value per sequence."""
-    if t is None and optional:
-        return None
-    if t is None or not t.is_cuda or t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous():
-        return f"{name} must be a contiguous int32 CUDA tensor [batch]"
-    return None
+def _kv8_refuse_devices(dev, *tensors):
+    if dev < 0 or any(t.get_device() < 0 for t in tensors):
+        raise RuntimeError("all tensors must be CUDA tensors")
+    raise RuntimeError("all tensors must be on the same device")
 
 
-def _kv8_check(msg) -> None:
-    if msg is not None:
-        raise RuntimeError(msg)
-
-
-def _kv8_cache_args(k_cache, v_cache, k_scale, v_scale, block_table):
-    """(cache pointers, format, pages, page size, table, its columns and row stride) as the library takes them."""
-    rows, blocks = block_table.shape
-    return (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            _KV8_FORMATS[k_cache.dtype], k_cache.shape[0], k_cache.shape[2], block_table.data_ptr(), blocks,
-            block_table.stride(0) if rows > 1 else blocks)
+def _kv8_lengths(name, t, batch, dev):
+    """The pointer of an int32 value per sequence."""
+    if (t is None or t.dtype is not torch.int32 or t.get_device() != dev or t.shape != (batch,)
+            or not t.is_contiguous()):
+        raise RuntimeError(f"{name} must be a contiguous int32 CUDA tensor [batch], on the cache's device")
+    return t.data_ptr()
 
 
 @traced
@@ -1179,38 +1180,31 @@ def kv8_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, *, c
     larger; where it grows, their bytes are rounded anew.  ``block_table[b]``
     lists the sequence's pages; no page may belong to two sequences that write
     to it in one call."""
-    _kv8_check(_kv8_cache_error(k_cache, v_cache, k_scale, v_scale, block_table)
-               or _kv8_new_error(k, v, k_cache, block_table) or _kv8_lengths_error("start", start, k.shape[0])
-               or _kv8_lengths_error("counts", counts, k.shape[0], optional=True))
     dev = k_cache.get_device()
-    if _MULTI_DEVICE:
-        _same_device(dev, k, v, v_cache, k_scale, v_scale, block_table, start, counts)
+    cache, H, D = _kv8_cache(dev, k_cache, v_cache, k_scale, v_scale, block_table)
+    if k.get_device() != dev or v.get_device() != dev:
+        _kv8_refuse_devices(dev, k, v)
+    if k.dim() != 4 or v.shape != k.shape:
+        raise RuntimeError("k and v must be [batch, kv_heads, new_tokens, head_dim]")
+    if k.dtype not in _KV8_DTYPES or v.dtype != k.dtype:
+        raise RuntimeError("k and v must both be float32, float16 or bfloat16")
+    B, heads, N, dim = k.shape
+    ks, vs = k.stride(), v.stride()
+    if k.numel() and not ks[3] == vs[3] == 1:
+        raise RuntimeError("k and v must be contiguous in head_dim")
+    if B != block_table.shape[0]:
+        raise RuntimeError("block_table must have one row per sequence")
+    if heads != H or dim != D:
+        raise RuntimeError("k and v must have the cache's heads and head_dim")
+    start_ptr = _kv8_lengths("start", start, B, dev)
+    counts_ptr = None if counts is None else _kv8_lengths("counts", counts, B, dev)
     if dev != _current_device():
         with torch.cuda.device(dev):
             return kv8_write(k, v, k_cache, v_cache, k_scale, v_scale, block_table, start, counts=counts)
-    B, H, N, D = k.shape
-    rc = lib().csahca_kv8_write(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], k.stride(0), k.stride(1), k.stride(2),
-                                v.stride(0), v.stride(1), v.stride(2),
-                                *_kv8_cache_args(k_cache, v_cache, k_scale, v_scale, block_table), start.data_ptr(),
-                                None if counts is None else counts.data_ptr(), B, H, N, D, _raw_stream(dev))
+    rc = lib().csahca_kv8_write(k.data_ptr(), v.data_ptr(), _DTYPES[k.dtype], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                                *cache, start_ptr, counts_ptr, B, H, N, D, _raw_stream(dev))
     if rc != 0:
         _rc(rc)
-
-
-def _kv8_new_error(k, v, k_cache, block_table):
-    if not (k.is_cuda and v.is_cuda):
-        return "k and v must be CUDA tensors"
-    if k.dim() != 4 or v.shape != k.shape:
-        return "k and v must be [batch, kv_heads, new_tokens, head_dim]"
-    if k.dtype not in _KV8_DTYPES or v.dtype != k.dtype:
-        return "k and v must both be float32, float16 or bfloat16"
-    if k.numel() and (k.stride(3) != 1 or v.stride(3) != 1):
-        return "k and v must be contiguous in head_dim"
-    if k.shape[0] != block_table.shape[0]:
-        return "block_table must have one row per sequence"
-    if k.shape[1] != k_cache.shape[1] or k.shape[3] != k_cache.shape[3]:
-        return "k and v must have the cache's heads and head_dim"
-    return None
 
 
 @traced
@@ -1219,46 +1213,50 @@ def kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, lengths, max_token
     ``[batch, kv_heads, max_tokens, head_dim]`` in ``dtype``: the positions from
     ``start[b]`` (int32; None: 0) on, 0 at and past ``lengths[b]``."""
     max_tokens = int(max_tokens)
-    _kv8_check(_kv8_cache_error(k_cache, v_cache, k_scale, v_scale, block_table)
-               or _kv8_lengths_error("lengths", lengths, block_table.shape[0])
-               or _kv8_lengths_error("start", start, block_table.shape[0], optional=True)
-               or (None if dtype in _KV8_DTYPES else f"unsupported dtype {dtype}")
-               or (None if max_tokens >= 0 else "max_tokens must be non-negative"))
     dev = k_cache.get_device()
-    if _MULTI_DEVICE:
-        _same_device(dev, v_cache, k_scale, v_scale, block_table, lengths, start)
+    cache, H, D = _kv8_cache(dev, k_cache, v_cache, k_scale, v_scale, block_table)
+    B = block_table.shape[0]
+    lengths_ptr = _kv8_lengths("lengths", lengths, B, dev)
+    start_ptr = None if start is None else _kv8_lengths("start", start, B, dev)
+    if dtype not in _KV8_DTYPES:
+        raise RuntimeError(f"unsupported dtype {dtype}")
+    if max_tokens < 0:
+        raise RuntimeError("max_tokens must be non-negative")
     if dev != _current_device():
         with torch.cuda.device(dev):
             return kv8_read(k_cache, v_cache, k_scale, v_scale, block_table, lengths, max_tokens, dtype=dtype,
                             start=start)
-    B, H, D = block_table.shape[0], k_cache.shape[1], k_cache.shape[3]
     k = torch.empty((B, H, max_tokens, D), dtype=dtype, device=k_cache.device)
     v = torch.empty_like(k)
-    rc = lib().csahca_kv8_read(*_kv8_cache_args(k_cache, v_cache, k_scale, v_scale, block_table),
-                               None if start is None else start.data_ptr(), lengths.data_ptr(), k.data_ptr(),
-                               v.data_ptr(), _DTYPES[dtype], B, H, max_tokens, D, _raw_stream(dev))
+    rc = lib().csahca_kv8_read(*cache, start_ptr, lengths_ptr, k.data_ptr(), v.data_ptr(), _DTYPES[dtype], B, H,
+                               max_tokens, D, _raw_stream(dev))
     if rc != 0:
         _rc(rc)
     return k, v
 
 
-def _kv8_q_error(q, k_cache, block_table, ranks):
-    if not q.is_cuda:
-        return "q must be a CUDA tensor"
+def _kv8_q(q, H, D, block_table, several):
+    """Checks q; returns (batch, queries, heads)."""
     if not q.is_contiguous():
-        return "q must be contiguous"
-    if q.dim() not in ranks:
-        return "q must be [batch, heads, head_dim]" + (" or [batch, queries, heads, head_dim]" if 4 in ranks else "")
+        raise RuntimeError("q must be contiguous")
+    shape = q.shape
+    if len(shape) == 3:
+        B, heads, dim = shape
+        queries = 1
+    elif several and len(shape) == 4:
+        B, queries, heads, dim = shape
+    else:
+        raise RuntimeError("q must be [batch, heads, head_dim]" +
+                           (" or [batch, queries, heads, head_dim]" if several else ""))
     if q.dtype not in _KV8_DTYPES:
-        return f"unsupported dtype {q.dtype}"
-    if q.shape[0] != block_table.shape[0]:
-        return "block_table must have one row per sequence"
-    if q.shape[-1] != k_cache.shape[3]:
-        return "q must have the cache's head_dim"
-    H = k_cache.shape[1]
-    if q.shape[-2] and (H == 0 or q.shape[-2] % H):
-        return "q heads must be a multiple of the cache's heads"
-    return None
+        raise RuntimeError(f"unsupported dtype {q.dtype}")
+    if B != block_table.shape[0]:
+        raise RuntimeError("block_table must have one row per sequence")
+    if dim != D:
+        raise RuntimeError("q must have the cache's head_dim")
+    if heads and (H == 0 or heads % H):
+        raise RuntimeError("q heads must be a multiple of the cache's heads")
+    return B, queries, heads
 
 
 @traced
@@ -1270,26 +1268,23 @@ def kv8_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, lengt
     ``lengths[b] - queries + 1 + i`` tokens).  ``heads`` is a multiple of the
     cache's heads.  A query that sees no token gives 0.  ``softmax_scale``
     defaults to ``1 / sqrt(head_dim)``."""
-    _kv8_check(_kv8_cache_error(k_cache, v_cache, k_scale, v_scale, block_table)
-               or _kv8_q_error(q, k_cache, block_table, (3, 4))
-               or _kv8_lengths_error("lengths", lengths, q.shape[0]))
     dev = q.get_device()
-    if _MULTI_DEVICE:
-        _same_device(dev, k_cache, v_cache, k_scale, v_scale, block_table, lengths)
+    cache, H, D = _kv8_cache(dev, k_cache, v_cache, k_scale, v_scale, block_table)
+    B, queries, heads = _kv8_q(q, H, D, block_table, True)
+    lengths_ptr = _kv8_lengths("lengths", lengths, B, dev)
     if dev != _current_device():
         with torch.cuda.device(dev):
             return kv8_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths,
                                       softmax_scale=softmax_scale)
-    B, heads, D = q.shape[0], q.shape[-2], q.shape[-1]
-    queries = q.shape[1] if q.dim() == 4 else 1
-    H, page, blocks = k_cache.shape[1], k_cache.shape[2], block_table.shape[1]
     out = torch.empty_like(q)
-    nbytes = _ws_bytes("csahca_kv8_decode_workspace_bytes", _DTYPES[q.dtype], B, queries, heads, H, D, page, blocks)
-    ws = _workspace(nbytes, q.device) if nbytes else None
+    nbytes = _ws_bytes("csahca_kv8_decode_workspace_bytes", _DTYPES[q.dtype], B, queries, heads, H, D, cache[6], cache[8])
+    # a workspace of the call's own: neither calls of several host threads on one
+    # stream nor captured graphs ever share one
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = lib().csahca_kv8_decode_forward(
-        q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, queries, heads, H, D,
-        *_kv8_cache_args(k_cache, v_cache, k_scale, v_scale, block_table), lengths.data_ptr(),
-        D ** -0.5 if softmax_scale is None else float(softmax_scale), _ptr(ws), nbytes, _raw_stream(dev))
+        q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, queries, heads, H, D, *cache, lengths_ptr,
+        D ** -0.5 if softmax_scale is None else float(softmax_scale), None if ws is None else ws.data_ptr(), nbytes,
+        _raw_stream(dev))
     if rc != 0:
         _rc(rc)
     return out
@@ -1306,40 +1301,33 @@ def kv8_csa_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, l
     Negative ids and tokens at or past ``lengths[b]`` are skipped; 0 when no
     token is left."""
     chunk_size = int(chunk_size)
-    _kv8_check(_kv8_cache_error(k_cache, v_cache, k_scale, v_scale, block_table)
-               or _kv8_q_error(q, k_cache, block_table, (3,)) or _kv8_lengths_error("lengths", lengths, q.shape[0])
-               or _kv8_chunks_error(chunk_indices, chunk_size, q, k_cache))
     dev = q.get_device()
-    if _MULTI_DEVICE:
-        _same_device(dev, k_cache, v_cache, k_scale, v_scale, block_table, lengths, chunk_indices)
+    cache, H, D = _kv8_cache(dev, k_cache, v_cache, k_scale, v_scale, block_table)
+    B, _, heads = _kv8_q(q, H, D, block_table, False)
+    lengths_ptr = _kv8_lengths("lengths", lengths, B, dev)
+    if chunk_indices.get_device() != dev:
+        _kv8_refuse_devices(dev, chunk_indices)
+    if not chunk_indices.is_contiguous():
+        raise RuntimeError("chunk_indices must be contiguous")
+    if chunk_indices.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("chunk_indices must be int32 or int64")
+    if chunk_indices.dim() != 3 or chunk_indices.shape[:2] != (B, H):
+        raise RuntimeError("chunk_indices must be [batch, kv_heads, top_k]")
+    if not chunk_size > 0:
+        raise RuntimeError("chunk_size must be positive")
     if dev != _current_device():
         with torch.cuda.device(dev):
             return kv8_csa_decode_forward(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, chunk_indices,
                                           chunk_size, softmax_scale=softmax_scale)
-    B, heads, D = q.shape
-    H, top_k = k_cache.shape[1], chunk_indices.shape[2]
+    top_k = chunk_indices.shape[2]
     out = torch.empty_like(q)
     nbytes = _ws_bytes("csahca_kv8_csa_decode_workspace_bytes", _DTYPES[q.dtype], B, heads, H, D, top_k, chunk_size)
-    ws = _workspace(nbytes, q.device) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     rc = lib().csahca_kv8_csa_decode_forward(
-        q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, heads, H, D,
-        *_kv8_cache_args(k_cache, v_cache, k_scale, v_scale, block_table), lengths.data_ptr(),
-        chunk_indices.data_ptr(), 0 if chunk_indices.dtype == torch.int32 else 1, top_k, chunk_size,
-        D ** -0.5 if softmax_scale is None else float(softmax_scale), _ptr(ws), nbytes, _raw_stream(dev))
+        q.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], B, heads, H, D, *cache, lengths_ptr,
+        chunk_indices.data_ptr(), 0 if chunk_indices.dtype is torch.int32 else 1, top_k, chunk_size,
+        D ** -0.5 if softmax_scale is None else float(softmax_scale), None if ws is None else ws.data_ptr(), nbytes,
+        _raw_stream(dev))
     if rc != 0:
         _rc(rc)
     return out
-
-
-def _kv8_chunks_error(chunk_indices, chunk_size, q, k_cache):
-    if not chunk_indices.is_cuda:
-        return "chunk_indices must be a CUDA tensor"
-    if not chunk_indices.is_contiguous():
-        return "chunk_indices must be contiguous"
-    if chunk_indices.dtype not in (torch.int32, torch.int64):
-        return "chunk_indices must be int32 or int64"
-    if chunk_indices.dim() != 3 or tuple(chunk_indices.shape[:2]) != (q.shape[0], k_cache.shape[1]):
-        return "chunk_indices must be [batch, kv_heads, top_k]"
-    if not chunk_size > 0:
-        return "chunk_size must be positive"
-    return None
