@@ -75,16 +75,32 @@ struct Split {
   int row_groups;
   int round;       // wavefronts over the tokens
   int min_tiles;   // 64-token tiles of a part, at least (a list: exactly)
-  int target_log2;
+  int even_log2, ragged_log2;  // workgroups over the tokens, at most about: lengths alike, ragged
   int64_t parts;   // parts over the batch, at most
   bool joined;     // whether a sequence may have several
 };
 
-
+// Each threshold with both sides measured (us; heads of 128 in bf16 unless said;
+// kernel + join where there is one):
+//   * more than 64 rows go to the kernel of many rows: 96 rows over 4 x 8192 tokens
+//     38 + 7 there, 43 + 9 with 32 rows a wavefront; 160 rows 46 + 9 / 67 + 6; up to
+//     64 they fit a workgroup of the other at 30 + 7.  (Heads of 64, 128 rows: 27 / 25.)
+//   * two row tiles a wavefront for 17 rows on, up to heads of 192: 32 rows over
+//     8 x 16384 tokens 54 / 58 with one, 64 rows 68 / 87, 64 rows of 192 97 / 122; of
+//     256, where the registers spill, 304 / 183.
+//   * up to four rounds of a workgroup's wavefronts go undivided, without the join:
+//     512 tokens 11.4 / 8.9 + 4.2, 1024 tokens 14 / 10.5 + 4.5, 2048 tokens 20 / 10 + 4.3.
+//   * lengths that are alike are divided among 2^8 workgroups, one a CU (32 rows over
+//     8 x 16384 tokens 64 + 4 with 2^8, 70 + 6 with 2^9, 82 + 8 with 2^10; single rows
+//     differ by 2), so 2^9 for lists too costs the join (27 + 4 / 28); ragged ones
+//     (uniform up to 32768) among 2^10, of a batch of 16 with 4 rows 74 + 6, 84 + 5
+//     with 2^9, 100 with 2^8; of more rows, whose partial results weigh more, 2^9 (32
+//     rows 62 + 5, 67 + 8 with 2^10) and in the kernel of many rows 2^8 (512 rows
+//     53 + 12, 82 + 41 with 2^10).
 Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t head_dim, int64_t tiles, bool list) {
   Split s;
   const int64_t row_tiles = ceil_div(rows, 16);
-  if (rows > 128 && dtype != CSAHCA_F32) {  // the kernel of many rows, 32 a wavefront
+  if (rows > 64 && dtype != CSAHCA_F32) {  // the kernel of many rows, 32 a wavefront
     s.tiles = 0;
     s.row_waves = kv8_rows_waves(head_dim);
     s.row_groups = static_cast<int>(ceil_div(row_tiles, 2 * s.row_waves));
@@ -96,13 +112,14 @@ Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t
     s.row_groups = static_cast<int>(ceil_div(waves, s.row_waves));
     s.round = kKv8Waves / s.row_waves;
   }
-  s.target_log2 = list || s.row_waves >= 4 ? 8 : 10;
+  s.even_log2 = 8;
+  s.ragged_log2 = s.tiles == 0 ? 8 : rows <= 16 ? 10 : 9;
   const int round = s.round;
-  // Up to four rounds of a workgroup's wavefronts go undivided, without the join.
   s.min_tiles = tiles <= 4 * round ? std::max(static_cast<int>(ceil_div(tiles, round)), 1) * round : round;
-  const int64_t target = int64_t{1} << s.target_log2, lanes = kv_heads * s.row_groups;
+  const int64_t target = int64_t{1} << (list ? s.even_log2 : s.ragged_log2);
+  const int64_t lanes = kv_heads * s.row_groups;
   if (list) {
-    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(tiles * batch * lanes / target + 1, s.min_tiles), round) * round);
+    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(ceil_div(tiles * batch * lanes, target), s.min_tiles), round) * round);
     s.parts = batch * ceil_div(tiles, s.min_tiles);
   } else {
     s.parts = std::min(target / lanes + batch, batch * std::max<int64_t>(ceil_div(tiles, s.min_tiles), 1));
@@ -122,22 +139,24 @@ int attend(Kv8Attend a, int format, int64_t tiles, void* workspace, size_t works
                  "too many query rows in one call");
   if (s.joined && (workspace == nullptr || workspace_bytes < workspace_of(s, a.c.kv_heads, a.rows, a.c.head_dim)))
     return fail(CSAHCA_ERR_WORKSPACE, "workspace too small for kv8 decode");
+  const int64_t brows = int64_t{a.rows} * a.c.kv_heads, lanes = kKv8Threads / (a.c.head_dim / 4);
+  a.join_lanes = static_cast<int32_t>(std::min(lanes, ceil_div(s.parts / a.batch, 4)));
+  const int64_t join_grid = ceil_div(brows, lanes / a.join_lanes) * a.batch;
+  CSAHCA_REQUIRE(!s.joined || join_grid <= UINT32_MAX / kKv8Threads, "too many query rows in one call");
   a.row_groups = s.row_groups;
   a.row_waves = s.row_waves;
   a.round = s.round;
   a.parts = static_cast<int32_t>(s.parts);
   a.min_tiles = s.min_tiles;
-  a.target_log2 = s.target_log2;
+  a.even_log2 = s.even_log2;
+  a.ragged_log2 = s.ragged_log2;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + s.parts * a.c.kv_heads * a.rows * a.c.head_dim;
   const int rc = format == CSAHCA_KV8_E4M3 ? kv8_attend_launch_e4m3(a, s.tiles, stream)
                                            : kv8_attend_launch_int8(a, s.tiles, stream);
   if (rc != CSAHCA_OK || !s.joined) return rc;
-  const int64_t brows = int64_t{a.rows} * a.c.kv_heads, lanes = kKv8Threads / (a.c.head_dim / 4);
-  a.join_lanes = static_cast<int32_t>(std::min(lanes, ceil_div(s.parts / a.batch, 4)));
-  return launch("kv8_join_kernel", kv8_join_kernel,
-                dim3(static_cast<uint32_t>(ceil_div(brows, lanes / a.join_lanes) * a.batch)), dim3(kKv8Threads), 0,
-                stream, a);
+  return launch("kv8_join_kernel", kv8_join_kernel, dim3(static_cast<uint32_t>(join_grid)), dim3(kKv8Threads), 0, stream,
+                a);
 }
 
 int check(const Kv8Cache& c, int dtype, int format, int64_t batch, int64_t queries, int64_t heads, int64_t kv_heads,

@@ -76,7 +76,8 @@ struct Kv8Attend {
   int32_t parts;       // parts of all sequences, at most
   int32_t round;       // wavefronts over the tokens, a power of two: a part has a multiple of as many tiles
   int32_t min_tiles;   // tiles of a part, at least
-  int32_t target_log2; // about 2^target_log2 workgroups over all
+  int32_t even_log2;   // workgroups over the tokens, at most about, where lengths are alike ...
+  int32_t ragged_log2; // ... and where they are not
   int32_t join_lanes;  // of a joining workgroup, thread groups that share a row's parts
   uint32_t page_groups;  // groups of 16 tokens of a page, 1 to 16 ...
   uint32_t page_magic;   // ... and 2^32 / that, rounded up
@@ -114,20 +115,26 @@ __device__ __forceinline__ int32_t kv8_tiles(const Kv8Attend& a, int32_t b) {
   return b < a.batch ? (kv8_length(a, b) + kKv8Tile - 1) / kKv8Tile : 0;
 }
 
-// Tiles of a part: one size for all sequences, from the lengths on the device,
-// so that ragged lengths spread evenly over about 2^target_log2 workgroups.
-// Whole rounds of the wavefronts that split the tokens.  Every wavefront works
-// it out by itself, a lane a sequence; `mine` is the lane's tiles of the last
-// 64 sequences (of all, where the batch is not larger).
+// Tiles of a part: one size for all sequences, from the lengths on the device, in
+// whole rounds of the wavefronts that split the tokens.  Lengths that are alike
+// are divided among 2^even_log2 workgroups, which run at once; ragged ones among
+// 2^ragged_log2, so that the last to run are short.  Every wavefront works it out
+// by itself, a lane a sequence; `mine` is the lane's tiles of the last 64
+// sequences (of all, where the batch is not larger).
 __device__ __forceinline__ int32_t kv8_part_size(const Kv8Attend& a, int32_t* mine) {
   const int lane = threadIdx.x % kWave;
   int64_t total = 0;
+  int32_t most = 0;
   for (int base = 0; base < a.batch; base += kWave) {
     *mine = kv8_tiles(a, base + lane);
     total += kv8_wave_sum(*mine);
+    most = max(most, *mine);
   }
-  const int64_t per = (total * a.c.kv_heads * a.row_groups) >> a.target_log2;
-  return (max(a.min_tiles, static_cast<int32_t>(per) + 1) + a.round - 1) & -a.round;
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) most = max(most, __float_as_int(xor_lanes(__int_as_float(most), d)));
+  const int log2 = static_cast<int64_t>(most) * a.batch <= total + total / 8 ? a.even_log2 : a.ragged_log2;
+  const int64_t per = (total * a.c.kv_heads * a.row_groups + (int64_t{1} << log2) - 1) >> log2;
+  return (max(a.min_tiles, static_cast<int32_t>(per)) + a.round - 1) & -a.round;
 }
 
 // The part of index `part` over all sequences, each of which has at least one
@@ -231,9 +238,11 @@ __device__ __forceinline__ uint64_t kv8_opaque(const void* p) {
   asm volatile("" : "+v"(a));
   return a;
 }
-template <typename V>
+template <typename V, bool kStream>
 __device__ __forceinline__ V kv8_load(uint64_t base, int offset) {
-  return *reinterpret_cast<const __attribute__((address_space(1))) V*>(base + offset);
+  const auto* p = reinterpret_cast<const __attribute__((address_space(1))) V*>(base + offset);
+  if constexpr (kStream) return __builtin_nontemporal_load(p);
+  return *p;
 }
 
 // The larger of three in one instruction (fmaxf twice also quiets each operand).
@@ -329,12 +338,21 @@ __device__ __forceinline__ void kv8_store4(const Kv8Attend& a, int64_t at, f32x4
 }
 
 // Workgroups of a CU: two while a wavefront's registers (K, V, the sums, q, scores
-// and weights) fit 256.
-template <int D, int NP, int NT>
-constexpr int kKv8Blocks = D / 4 * (2 + NT) + NP * NT * D / 8 + 16 * NT + 8 * NP * NT <= 216 ? 2 : 1;
+// and weights, counted in the second line) fit 256 beside some 70 others: 64 rows of
+// 96 over 8 x 16384 tokens 51 us, one workgroup 58; of 128, which do not fit, 88 / 68;
+// 64 rows of 192 one by one 126 / 122.  In between are f32 rows of 128: 16 rows
+// 53 / 50, 32 rows, which share the loads, 34 / 38.
+template <int D, int NP, int NT, bool kStream>
+constexpr int kKv8Blocks =
+    D / 4 * (2 + NT) + NP * NT * D / 8 + 16 * NT + 8 * NP * NT <= (kStream ? 180 : 190) ? 2 : 1;
 
-template <int D, typename F, bool kF32, int NT>
-__global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) void kv8_attend_kernel(const Kv8Attend a) {
+// kStream: no other wavefront reads a tile (one over the rows), and its loads go
+// past the caches: 32 x 32768 tokens 370 us without and 344 with (6.2 TB/s), 16 ragged
+// 78.6 / 73.4, 32 rows over 8 x 16384 tokens 59 / 54, of 192 84 / 77 (of 64 27 / 28);
+// where wavefronts share tiles it costs (heads of 256 in 4 wavefronts of 16 rows:
+// 57.7 / 81.3).
+template <int D, typename F, bool kF32, int NT, bool kStream>
+__global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStream>)) void kv8_attend_kernel(const Kv8Attend a) {
   constexpr int NP = kF32 ? 3 : 1;         // operands that make up a value of q or a weight
   constexpr int kSteps = D / 32;           // matrix instructions over D
   constexpr int kWide = D / 64;            // 16-byte loads of a K row
@@ -402,14 +420,14 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT>)) voi
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int w = 0; w < kWide; ++w) kw[t][w] = kv8_load<u32x4_t>(wide, 4 * t * D + 64 * w);
-      if constexpr (kTail) kt[t] = kv8_load<u32x2_t>(tail, 4 * t * D);
+      for (int w = 0; w < kWide; ++w) kw[t][w] = kv8_load<u32x4_t, kStream>(wide, 4 * t * D + 64 * w);
+      if constexpr (kTail) kt[t] = kv8_load<u32x2_t, kStream>(tail, 4 * t * D);
     }
   };
   const auto load_v = [&](uint32_t at) {
     const uint64_t base = kv8_opaque(vbase + static_cast<int64_t>(at) * (kKv8Group * D));
 #pragma unroll
-    for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = kv8_load<u32x4_t>(base, dt * 16 * kKv8Group);
+    for (int dt = 0; dt < kDTiles; ++dt) vw[dt] = kv8_load<u32x4_t, kStream>(base, dt * 16 * kKv8Group);
   };
 
   // The pages of the segment's sub-blocks, then this wavefront's first loads and
@@ -1168,16 +1186,21 @@ int kv8_attend_launch(const Kv8Attend& a, int tiles, hipStream_t stream) {
   const auto go = [&](auto kernel) {
     return launch("kv8_attend_kernel", kernel, grid, dim3(kKv8Threads), 0, stream, a);
   };
+  const bool alone = a.row_waves == 1;
   const auto by_tiles = [&](auto dim) {
     constexpr int D = decltype(dim)::value;
-    if (a.dtype == CSAHCA_F32) return go(kv8_attend_kernel<D, F, true, 1>);
+    if (a.dtype == CSAHCA_F32)
+      return alone ? go(kv8_attend_kernel<D, F, true, 1, true>) : go(kv8_attend_kernel<D, F, true, 1, false>);
     if (tiles == 0)
       return launch("kv8_attend_rows_kernel", kv8_attend_rows_kernel<D, F>, grid, dim3(kv8_rows_waves(D) * kWave), 0, stream,
                     a);
     if constexpr (D <= kKv8TwoTilesDim) {
-      if (tiles == 2) return go(kv8_attend_kernel<D, F, false, 2>);
+      if (tiles == 2)
+        return alone ? go(kv8_attend_kernel<D, F, false, 2, true>) : go(kv8_attend_kernel<D, F, false, 2, false>);
+    } else {
+      if (!alone) return go(kv8_attend_kernel<D, F, false, 1, false>);
     }
-    return go(kv8_attend_kernel<D, F, false, 1>);
+    return go(kv8_attend_kernel<D, F, false, 1, true>);
   };
   switch (a.c.head_dim / 32) {
     case 1: return by_tiles(std::integral_constant<int, 32>{});
