@@ -8,14 +8,15 @@ namespace csahca {
 namespace {
 
 // The rows (batch, K/V head, row) of sequences that have several parts:
-// out = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p, M = max m_p.  A thread
+// out = 2^(M - S) sum_p 2^(m_p - M) O_p / sum_p 2^(s_p - S) l_p, M = max m_p, S = max
+// s_p, the maxima of the parts' numerators and sums.  A thread
 // takes four dimensions of a row and every join_lanes-th part; a row's parts are
 // in flight together, up to four a thread (a wavefront a row and four parts a
 // round trip took 22 us for the 32 parts of 8192 tokens of 8 heads, this 4.6).
 // The order of the sums is fixed by the split alone.
 __global__ __launch_bounds__(kKv8Threads) void kv8_join_kernel(const Kv8Attend a) {
   __shared__ f32x4_t sums[kKv8Threads];
-  __shared__ float tops[kKv8Threads], totals[kKv8Threads];
+  __shared__ float tops[kKv8Threads], stops[kKv8Threads], totals[kKv8Threads];
   const int32_t D = a.c.head_dim, wide = D / 4, lanes = kKv8Threads / wide;
   const int32_t per = lanes / a.join_lanes;  // rows of a workgroup, all of one sequence
   const int64_t brows = static_cast<int64_t>(a.c.kv_heads) * a.rows, groups = (brows + per - 1) / per;
@@ -29,43 +30,45 @@ __global__ __launch_bounds__(kKv8Threads) void kv8_join_kernel(const Kv8Attend a
   const int32_t h = static_cast<int32_t>(hr / a.rows), r = static_cast<int32_t>(hr % a.rows);
   const int64_t step = static_cast<int64_t>(a.c.kv_heads) * a.rows;
   const int64_t slot0 = (static_cast<int64_t>(first) * a.c.kv_heads + h) * a.rows + r;
-  float top = -FLT_MAX, total = 0.f;
+  float top = -FLT_MAX, stop = -FLT_MAX, total = 0.f;
   f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+  const auto add = [&](float m, float ms, float l, f32x4_t o) {
+    const float up = fmaxf(top, m), sup = fmaxf(stop, ms);
+    total = total * fast_exp2(stop - sup) + l * fast_exp2(ms - sup);
+    acc = acc * fast_exp2(top - up) + o * fast_exp2(m - up);
+    top = up;
+    stop = sup;
+  };
   if (mine) {
     for (int p0 = lane; p0 < count; p0 += 4 * a.join_lanes) {
-      float2 ml[4];
+      float4 ml[4];
       f32x4_t o[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // behind the last part: that part again, unused
         const int64_t slot = slot0 + min(p0 + i * a.join_lanes, count - 1) * step;
-        ml[i] = reinterpret_cast<const float2*>(a.part_ml)[slot];
+        ml[i] = reinterpret_cast<const float4*>(a.part_ml)[slot];
         o[i] = *reinterpret_cast<const f32x4_t*>(a.part_o + slot * D + d);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (p0 + i * a.join_lanes >= count) break;
-        const float up = fmaxf(top, ml[i].x), was = fast_exp2(top - up), is = fast_exp2(ml[i].x - up);
-        total = total * was + ml[i].y * is;
-        acc = acc * was + o[i] * is;
-        top = up;
+        add(ml[i].x, ml[i].y, ml[i].z, o[i]);
       }
     }
   }
   tops[threadIdx.x] = top;
+  stops[threadIdx.x] = stop;
   totals[threadIdx.x] = total;
   sums[threadIdx.x] = acc;
   __syncthreads();
   if (!mine || lane > 0) return;
   for (int i = 1; i < a.join_lanes; ++i) {
     const int at = i * wide + threadIdx.x;
-    const float up = fmaxf(top, tops[at]), was = fast_exp2(top - up), is = fast_exp2(tops[at] - up);
-    total = total * was + totals[at] * is;
-    acc = acc * was + sums[at] * is;
-    top = up;
+    add(tops[at], stops[at], totals[at], sums[at]);
   }
-  const float inv = total != 0.f ? 1.0f / total : 0.f;
   const int64_t heads = static_cast<int64_t>(a.c.kv_heads) * a.group;
-  kv8_store4(a, ((b * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D + d, acc * inv);
+  kv8_store4(a, ((b * a.queries + r / a.group) * heads + h * a.group + r % a.group) * D + d,
+             kv8_result(acc, total, top - stop));
 }
 
 // How a call is laid out over workgroups, from its sizes alone.
@@ -129,7 +132,7 @@ Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t
 }
 
 size_t workspace_of(const Split& s, int64_t kv_heads, int64_t rows, int64_t head_dim) {
-  return s.joined ? static_cast<size_t>(s.parts * kv_heads * rows * (head_dim + 2)) * sizeof(float) : 0;
+  return s.joined ? static_cast<size_t>(s.parts * kv_heads * rows * (head_dim + 4)) * sizeof(float) : 0;
 }
 
 int attend(Kv8Attend a, int format, int64_t tiles, void* workspace, size_t workspace_bytes, hipStream_t stream) {

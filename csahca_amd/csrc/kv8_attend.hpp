@@ -26,12 +26,19 @@
 // so p V is in units of the largest p vs so far whatever the scales are, and the
 // softmax's sum takes p / vs (by a third small product, as if V's byte were 1,
 // whose rows keep the sub-blocks apart).  p is rounded to f16's 11 bits.  It is
-// held times 2^11 and m moves only when a score passes it by 4: the sums are
-// rarely rescaled, p stays at most 2^15, and what is lost of a weight for want of
-// exponent is at most 2^-36 of the largest weight.
+// held times 2^12; m is an integer (so that differences of such maxima are exact) and
+// moves only when a score passes it by 3: the sums are rarely rescaled, p stays at
+// most 2^15, and what is lost of a weight for want of exponent is at most 2^-36 of
+// the largest p vs.  For the sum that is 2^-36 of its largest weight times the ratio
+// of two V scales.  Where those of a part differ by more than 2^10 (a page of zeros
+// has the least scale there is), or are so small that p / vs would overflow, the sum
+// is taken by 16 more exponentials a lane and tile, beside a maximum of the scores
+// alone; sums and their maxima are kept and joined apart from the numerators'
+// (which costs the rest 0.3 us a call).
 //
 // Beside f32 values the operands are bf16, as wide as f32: q and p as three bf16
-// each, 24 bits, of which nothing is lost.
+// each, 24 bits, of which nothing is lost.  Rows of q beyond 2^60 are scaled to
+// that, so that products with bytes do not overflow before K's scale is applied.
 #pragma once
 
 #include <cfloat>
@@ -47,8 +54,11 @@ constexpr int kKv8SegTiles = 256;  // tiles whose pages a workgroup looks up at 
 constexpr int kKv8Lookups = kKv8SegTiles * 4 / kKv8Threads;  // sub-blocks of a segment a thread
 constexpr int kKv8GridRows = 32768;   // of a launch: its y dimension, the rest in z
 constexpr int kKv8TwoTilesDim = 192;  // head sizes up to which a wavefront's registers hold two row tiles
-constexpr float kKv8PShift = 11.0f;  // a weight is held times 2^11 ...
-constexpr float kKv8Slack = 4.0f;    // ... and may pass the running maximum by 2^4
+constexpr float kKv8PShift = 12.0f;  // a weight is held times 2^12 ...
+constexpr float kKv8Slack = 3.0f;    // ... and may pass the running maximum by 2^3
+constexpr float kKv8Near = 3.0f;     // V scales of a wavefront's look-up are near within 2^3 of one of them ...
+constexpr float kKv8NearRefs = 4.0f;   // ... and those of a part if those ones are within 2^4 of each other
+constexpr float kKv8NearLeast = -80.0f;  // and none is below 2^-80, where the sum of weights / scale would overflow
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -82,7 +92,7 @@ struct Kv8Attend {
   uint32_t page_groups;  // groups of 16 tokens of a page, 1 to 16 ...
   uint32_t page_magic;   // ... and 2^32 / that, rounded up
   float scale_log2;
-  float* part_ml;      // [parts, kv_heads, rows, 2]
+  float* part_ml;      // [parts, kv_heads, rows, 4]: m, the sum's maximum, the sum, unused
   float* part_o;       // [parts, kv_heads, rows, D]
 };
 
@@ -252,6 +262,36 @@ __device__ __forceinline__ float kv8_max3(float a, float b, float c) {
   return r;
 }
 
+// log2 of V scales, of a lane's sub-blocks or a part's: the least and the largest.
+struct Kv8Range {
+  float lo = FLT_MAX, hi = -FLT_MAX;
+};
+
+// One of a wavefront's, +inf where they are not near that one, NaN where there are none.
+__device__ __forceinline__ float kv8_scale_ref(const Kv8Range& lane) {
+  const uint64_t has = __ballot(lane.hi > -FLT_MAX);
+  if (has == 0) return __builtin_nanf("");
+  const float ref = __int_as_float(
+      __builtin_amdgcn_readlane(__float_as_int(lane.hi), __ffsll(static_cast<unsigned long long>(has)) - 1));
+  const bool far = lane.lo < fmaxf(ref - kKv8Near, kKv8NearLeast) || lane.hi > ref + kKv8Near;
+  return __ballot(far) ? __builtin_inff() : ref;
+}
+
+// Whether the V scales of a part are far apart, with the refs of N more wavefronts.
+template <int N>
+__device__ __forceinline__ bool kv8_far_scales(const float* refs, Kv8Range* part) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const f32x4_t ref = *reinterpret_cast<const f32x4_t*>(refs + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      part->lo = fminf(part->lo, ref[k]);
+      part->hi = fmaxf(part->hi, ref[k]);
+    }
+  }
+  return __ballot(part->hi - part->lo > kKv8NearRefs) != 0;
+}
+
 // 0x80 in each byte that is an e4m3 NaN.
 __device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -337,6 +377,14 @@ __device__ __forceinline__ void kv8_store4(const Kv8Attend& a, int64_t at, f32x4
   }
 }
 
+// The sums 2^up acc / total, 0 where there are none.
+__device__ __forceinline__ f32x4_t kv8_result(f32x4_t acc, float total, float up) {
+  acc *= total != 0.f ? 1.0f / total : 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = __builtin_ldexpf(acc[i], static_cast<int>(up));
+  return acc;
+}
+
 // Workgroups of a CU: two while a wavefront's registers (K, V, the sums, q, scores
 // and weights, counted in the second line) fit 256 beside some 70 others: 64 rows of
 // 96 over 8 x 16384 tokens 51 us, one workgroup 58; of 128, which do not fit, 88 / 68;
@@ -362,7 +410,9 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
   constexpr size_t kMergeBytes = sizeof(float) * kKv8Waves * 16 * kRowPad;
   constexpr size_t kSubBytes = 20 * kKv8SegTiles * 4;
   __shared__ __attribute__((aligned(16))) char lds[kMergeBytes > kSubBytes ? kMergeBytes : kSubBytes];
-  __shared__ float lds_ml[kKv8Waves][16][2];
+  __shared__ float4 lds_ml[kKv8Waves][16];  // the maximum, the sum's maximum, the sum
+  __shared__ float lds_ms[kKv8Waves][NT * 16];  // where V scales are far apart, the sums' maxima
+  __shared__ __attribute__((aligned(16))) float refs[kKv8Waves];  // of a segment's V scales
   uint2* sub_at = reinterpret_cast<uint2*>(lds);                          // index, valid tokens
   float2* sub_scale = reinterpret_cast<float2*>(lds) + kKv8SegTiles * 4;  // K scale, log2 of the V scale
   float* sub_inv = reinterpret_cast<float*>(lds) + kKv8SegTiles * 16;     // 1 / V scale
@@ -432,20 +482,20 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
 
   // The pages of the segment's sub-blocks, then this wavefront's first loads and
   // the sub-blocks' scales, which only the scores wait for.
-  float ks[kKv8Lookups], vs[kKv8Lookups];
+  float ks[kKv8Lookups], vs[kKv8Lookups];  // vs 0: none
   const int32_t first = wave % token_waves;
   const auto look_up = [&](int32_t seg, int32_t tiles) {
 #pragma unroll
     for (int i = 0; i < kKv8Lookups; ++i) {
       const int at = i * kKv8Threads + threadIdx.x;
       ks[i] = 0.f;
-      vs[i] = 1.f;
+      vs[i] = 0.f;
       if (at < tiles * 4) {
         const Kv8Sub sub = kv8_resolve(a, b, h, len, static_cast<uint32_t>(seg) * 4 + at);
         sub_at[at] = make_uint2(sub.at, sub.lohi);
         if (sub.scale >= 0) {
           ks[i] = a.c.k_scale[sub.scale];
-          vs[i] = a.c.v_scale[sub.scale];
+          vs[i] = fmaxf(a.c.v_scale[sub.scale], FLT_MIN);
         }
       }
     }
@@ -480,23 +530,23 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
         widen16<bf16>(make_uint4(w[0], w[1], w[2], w[3]), v[k]);
       }
     }
+    // times 2^down: 16-bit rows to below 2^15, f32 rows beyond 2^60 to that, so that no product overflows
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+    top = fmaxf(top, xor_lanes(top, 16));
+    top = fmaxf(top, xor_lanes(top, 32));
     int e2 = 15;
-    if constexpr (!kF32) {
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
-      top = fmaxf(top, xor_lanes(top, 16));
-      top = fmaxf(top, xor_lanes(top, 32));
-      if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
-    }
+    if (top > 0.f && top < __builtin_inff()) (void)frexpf(top, &e2);
+    const int down = kF32 ? min(60 - e2, 0) : 15 - e2;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = kF32 ? v[k][e] * sign : __builtin_ldexpf(v[k][e] * sign, 15 - e2);
+      for (int e = 0; e < 8; ++e) v[k][e] = __builtin_ldexpf(v[k][e] * sign, down);
       kv8_split<kF32>(v[k], q[nt][k]);
     }
-    rc[nt] = __builtin_ldexpf(fabsf(a.scale_log2), e2 - 15);
+    rc[nt] = __builtin_ldexpf(fabsf(a.scale_log2), -down);
     m[nt] = -FLT_MAX;  // finite: a row of NaN scores still reaches the sums
     l[nt] = 0.f;
 #pragma unroll
@@ -508,18 +558,30 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
   for (int i = 0; i < 4; ++i) ones[i] = n != g ? 0u : kF32 ? 0x3f803f80u : 0x3c003c00u;
   if constexpr (!kEarly) look_up(part.begin, min(end - part.begin, kKv8SegTiles));
 
+  bool far = false;
+  Kv8Range scales;
   for (int32_t seg = part.begin; seg < end;) {
     const int32_t seg_end = min(end - seg, kKv8SegTiles);
+    Kv8Range range;
 #pragma unroll
     for (int i = 0; i < kKv8Lookups; ++i) {
+      if (i * kKv8Threads >= seg_end * 4) break;
       const int at = i * kKv8Threads + threadIdx.x;
+      const float lv = __builtin_amdgcn_logf(vs[i]);
+      if (vs[i] > 0.f) range = {fminf(range.lo, lv), fmaxf(range.hi, lv)};
       if (at < seg_end * 4) {
-        const float lv = __builtin_amdgcn_logf(fmaxf(vs[i], FLT_MIN));
-        sub_scale[at] = make_float2(ks[i], lv);
-        sub_inv[at] = fast_exp2(-lv);
+        sub_scale[at] = make_float2(ks[i], vs[i] > 0.f ? lv : 0.f);
+        sub_inv[at] = vs[i] > 0.f ? fast_exp2(-lv) : 0.f;
       }
     }
+    const float ref = kv8_scale_ref(range);
+    if (lane == 0) refs[wave] = ref;
     lds_barrier();
+    if (kv8_far_scales<kKv8Waves>(refs, &scales) && !far) {
+      far = true;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) lds_ms[wave][nt * 16 + n] = m[nt];
+    }
 
     // One tile; its successor's K and V are loaded as its own are done with.
     const auto tile_step = [&](int32_t tile, auto more) {
@@ -593,7 +655,7 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
           for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
             for (int w = 0; w < 4; ++w) any |= kv8_nan_bytes(vw[dt][w]);
-          if (__ballot(any != 0)) {
+          if (__builtin_expect(__ballot(any != 0) != 0, 0)) {
             u32x4_t seen[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -633,7 +695,7 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
       bool up = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        c[nt] = fmaxf(scale.x * rc[nt], 1e-30f);
+        c[nt] = fmaxf(scale.x * rc[nt], FLT_MIN);
         float most = s[nt][3][3];
 #pragma unroll
         for (int i = 0; i < 14; i += 2) most = kv8_max3(most, s[nt][i / 4][i % 4], s[nt][(i + 1) / 4][(i + 1) % 4]);
@@ -646,12 +708,29 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
       if (__ballot(up)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          top[nt] = fmaxf(top[nt], m[nt]);
+          top[nt] = ceilf(fmaxf(top[nt], m[nt]));
           const float fix = fast_exp2(m[nt] - top[nt]);
-          l[nt] *= fix;
+          if (!far) l[nt] *= fix;
 #pragma unroll
           for (int dt = 0; dt < kDTiles; ++dt) o[nt][dt] *= fix;
           m[nt] = top[nt];
+        }
+      }
+      if (__builtin_expect(far, 0)) {
+        // The weights for the sum by themselves, beside their own maximum.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float most = -FLT_MAX;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) most = fmaxf(most, s[nt][i / 4][i % 4] * c[nt]);
+          most = fmaxf(most, xor_lanes(most, 16));
+          most = fmaxf(most, xor_lanes(most, 32));
+          const float was = lds_ms[wave][nt * 16 + n], up = fmaxf(was, ceilf(most));
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum += fast_exp2(fmaf(s[nt][i / 4][i % 4], c[nt], kKv8PShift - up));
+          l[nt] = fmaf(l[nt], fast_exp2(was - up), sum);
+          lds_ms[wave][nt * 16 + n] = up;
         }
       }
       const f32x4_t inv_vs = *reinterpret_cast<const f32x4_t*>(sub_inv + tile * 4);
@@ -670,7 +749,7 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
           for (int i = 0; i < NP; ++i) sum = kv8_mfma<kF32>(ones, pa[nt][half][i], sum);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[nt] = fmaf(sum[i], inv_vs[i], l[nt]);
+        for (int i = 0; i < 4; ++i) l[nt] = fmaf(sum[i], far ? 0.f : inv_vs[i], l[nt]);
       }
 #pragma unroll
       for (int dt = 0; dt < kDTiles; dt += 2) {
@@ -713,8 +792,7 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
     for (int dt = 0; dt < kDTiles; ++dt)
       *reinterpret_cast<f32x4_t*>(merge + (wave * 16 + n) * kRowPad + dt * 16 + g * 4) = o[nt][dt];
     if (g == 0) {
-      lds_ml[wave][n][0] = m[nt];
-      lds_ml[wave][n][1] = sum;
+      lds_ml[wave][n] = make_float4(m[nt], far ? lds_ms[wave][nt * 16 + n] : m[nt], sum, 0.f);
     }
     __syncthreads();
     // thread: (row wavefront, row, four dimensions)
@@ -722,24 +800,26 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
       const int d = i % (D / 4) * 4, row = i / (D / 4) % 16, w0 = i / (D / 4 * 16) * token_waves;
       const int32_t r = (rg * a.row_waves + w0 / token_waves) * (NT * 16) + nt * 16 + row;
       if (r >= a.rows) continue;
-      float top = -FLT_MAX, total = 0.f;
-      for (int w = 0; w < token_waves; ++w) top = fmaxf(top, lds_ml[w0 + w][row][0]);
+      float top = -FLT_MAX, stop = -FLT_MAX, total = 0.f;
+      for (int w = 0; w < token_waves; ++w) {
+        top = fmaxf(top, lds_ml[w0 + w][row].x);
+        stop = fmaxf(stop, lds_ml[w0 + w][row].y);
+      }
       f32x4_t acc{0.f, 0.f, 0.f, 0.f};
       for (int w = 0; w < token_waves; ++w) {
-        const float fix = fast_exp2(lds_ml[w0 + w][row][0] - top);
-        total = fmaf(lds_ml[w0 + w][row][1], fix, total);
-        acc += *reinterpret_cast<const f32x4_t*>(merge + ((w0 + w) * 16 + row) * kRowPad + d) * fix;
+        const float4 ml = lds_ml[w0 + w][row];
+        total = fmaf(ml.z, fast_exp2(ml.y - stop), total);
+        acc += *reinterpret_cast<const f32x4_t*>(merge + ((w0 + w) * 16 + row) * kRowPad + d) * fast_exp2(ml.x - top);
       }
       if (part.count > 1) {
         const int64_t slot = (static_cast<int64_t>(part_index) * a.c.kv_heads + h) * a.rows + r;
         *reinterpret_cast<f32x4_t*>(a.part_o + slot * D + d) = acc;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, total);
+        if (d == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * slot) = make_float4(top, stop, total, 0.f);
       } else {
-        const float inv = total != 0.f ? 1.0f / total : 0.f;
         const int32_t qi = a.queries == 1 ? 0 : r / a.group;
         const int64_t at =
             ((static_cast<int64_t>(b) * a.queries + qi) * heads + h * a.group + (r - qi * a.group)) * D + d;
-        kv8_store4(a, at, acc * inv);
+        kv8_store4(a, at, kv8_result(acc, total, top - stop));
       }
     }
   }
@@ -792,6 +872,8 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
   __shared__ uint64_t sub_cut[2][kWaves];          // sub-blocks that are not whole, a bit each
   __shared__ uint16_t nans[2][D][4];               // tokens of a sub-block whose V is NaN ...
   __shared__ uint32_t nan_at[2][kWaves];           // ... and whether a wavefront found any
+  __shared__ float lds_ms[kWaves][32];  // where V scales are far apart, the sums' maxima
+  __shared__ __attribute__((aligned(16))) float refs[2][kWaves];  // of a segment's V scales
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n = lane % 32, g = lane / 32;
@@ -859,13 +941,16 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
     sub_at[buf][threadIdx.x] = make_uint2(sub.at, sub.lohi);
     const uint64_t cut = __ballot(sub.lohi != kKv8Whole);
     if (lane == 0) sub_cut[buf][wave] = cut;
-    float ks = 0.f, vs = 1.f;
+    float ks = 0.f, lv = 0.f;
+    Kv8Range range;
     if (sub.scale >= 0) {
       ks = a.c.k_scale[sub.scale];
-      vs = a.c.v_scale[sub.scale];
+      lv = __builtin_amdgcn_logf(fmaxf(a.c.v_scale[sub.scale], FLT_MIN));
+      range = {lv, lv};
     }
-    const float lv = __builtin_amdgcn_logf(fmaxf(vs, FLT_MIN));
     sub_scale[buf][threadIdx.x] = make_float4(ks, lv, fast_exp2(-lv), 0.f);
+    const float ref = kv8_scale_ref(range);
+    if (lane == 0) refs[buf][wave] = ref;
   };
   // Entry of a tile's sub-block s (tiles are counted from the part's first).
   const auto entry = [](int32_t tile, int s) { return tile % kTiles * 4 + s; };
@@ -980,7 +1065,7 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float4 e = sub_scale[tile / kTiles % 2][entry(tile, 2 * u + g)];
-      x.c[u] = fmaxf(e.x * rc, 1e-30f);  // not 0, so that a masked score stays -inf
+      x.c[u] = fmaxf(e.x * rc, FLT_MIN);  // not 0, so that a masked score stays -inf
       x.lv[u] = e.y;
       x.inv[u] = e.z;
     }
@@ -997,9 +1082,16 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
   const int32_t tiles = end - part.begin;
   Scale now;
   float top = 0.f;  // of the tile's scores
+  bool far = false;
+  Kv8Range scales;
   const auto step = [&](int32_t tile, f32x16_t (&s)[2], f32x16_t (&t)[2]) {
-    if (tile % kTiles == 0 && tile + kTiles < tiles)
-      look_up(part.begin + tile + kTiles, tile / kTiles % 2 ^ 1);
+    if (tile % kTiles == 0) {
+      if (kv8_far_scales<kWaves>(refs[tile / kTiles % 2], &scales) && !far) {
+        far = true;
+        lds_ms[wave][n] = m;
+      }
+      if (tile + kTiles < tiles) look_up(part.begin + tile + kTiles, tile / kTiles % 2 ^ 1);
+    }
     const int32_t next = min(tile + 1, tiles - 1);
     const uint32_t cut = cut_of(next);
     constexpr int kAhead = 3;  // operands read ahead of their product
@@ -1010,12 +1102,31 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ready[i] = k_operand(i);
     if (__ballot(top > m + kKv8Slack)) {
-      top = fmaxf(top, m);
+      top = ceilf(fmaxf(top, m));
       const float fix = fast_exp2(m - top);
-      l *= fix;
+      if (!far) l *= fix;
 #pragma unroll
       for (int dt = 0; dt < kChunks; ++dt) o[dt] *= fix;
       m = top;
+    }
+
+    if (__builtin_expect(far, 0)) {
+      // The weights for the sum by themselves, beside their own maximum.
+      float most = -FLT_MAX;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[u][i] * now.c[u]);
+      most = fmaxf(most, xor_lanes(most, 32));
+      const float was = lds_ms[wave][n], up = fmaxf(was, ceilf(most));
+      float own = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) own += fast_exp2(fmaf(s[u][i], now.c[u], kKv8PShift - up));
+      l = fmaf(l, fast_exp2(was - up), own);
+      lds_ms[wave][n] = up;
+      now.inv[0] = now.inv[1] = 0.f;  // and none of these
     }
 
     // the weights, beside the next tile's scores
@@ -1155,6 +1266,7 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
   }
 
   l += xor_lanes(l, 32);
+  const float ms = far ? lds_ms[wave][n] : m;
   if (row0 + n >= a.rows) return;
   if (part.count > 1) {
     const int64_t slot = (static_cast<int64_t>(part_index) * a.c.kv_heads + h) * a.rows + r;
@@ -1164,15 +1276,14 @@ __global__ __launch_bounds__(kv8_rows_waves(D) * kWave) void kv8_attend_rows_ker
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4_t*>(a.part_o + slot * D + dt * 32 + 8 * i + 4 * g) =
             f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
-    if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(m, l);
+    if (g == 0) *reinterpret_cast<float4*>(a.part_ml + 4 * slot) = make_float4(m, ms, l, 0.f);
   } else {
-    const float inv = l != 0.f ? 1.0f / l : 0.f;
 #pragma unroll
     for (int dt = 0; dt < kChunks; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         kv8_store4(a, q_at + dt * 32 + 8 * i + 4 * g,
-                   f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]} * inv);
+                   kv8_result(f32x4_t{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]}, l, m - ms));
   }
 }
 

@@ -65,9 +65,11 @@ def bound(want, mass, size, dtype, D, n, peak):
     * the result: half a step of its type, which below the least normal value is
       half the least subnormal (f16: 2^-25);
     * every weight p: beside 16-bit values one rounding to f16's 11 bits, and where
-      f16 has no exponent for it half its least step: weights are held times 2^11
+      f16 has no exponent for it half its least step: weights are held times 2^12
       beside the largest, the step is 2^-24, so 2^-36 of the largest weight a token,
-      n 2^-36 ``peak`` in all; beside f32 24 bits and nothing lost;
+      n 2^-36 ``peak`` in all; beside f32 24 bits and nothing lost.  "Largest" is
+      by p times its page's V scale; where those differ by up to 2^10 the sum's
+      weights are the same ones, so it may miss n 2^-26 of itself;
     * p's own relative error, twice (numerator, sum): the score's |q| |k| products
       in fp32 (D + 8 roundings), 4 roundings of a score of that size and the
       exponential's two;
@@ -75,7 +77,7 @@ def bound(want, mass, size, dtype, D, n, peak):
       their rescalings."""
     half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     p_bits = 2.0 ** -23 if dtype == F32 else 2.0 ** -11
-    lost = 0.0 if dtype == F32 else n * peak * 2.0 ** -36
+    lost = 0.0 if dtype == F32 else n * (peak * 2.0 ** -36 + np.abs(want) * 2.0 ** -26)
     score = size[..., None] * (D + 12) * 2.0 ** -24 + 2.0 ** -21
     sums = (64 + n / 16) * 2.0 ** -24
     return half * np.abs(want) + mass * (p_bits + 2 * score + 2 * sums) + lost + least
@@ -395,6 +397,76 @@ def test_attend_large_and_small_queries():
     q[2] = 0
     for b, e in enumerate((100, -100, 0, 20, -30)):
         check_attend(q[b : b + 1], cache, cache, table[b : b + 1], lengths[b : b + 1], softmax_scale=2.0 ** (-e - 3))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attend_queries_whose_products_pass_fp32(dtype):
+    """q near the type's largest value over pages of tiny keys: the scores are moderate, q times a byte is not."""
+    q, cache, _, table, lengths = attend_case(2, 1, 2, 2, 64, 32, (70, 33), E4M3, dtype, seed=13)
+    cache.k_scale.fill_(2.0 ** -120)
+    q = (q.float().clamp(-3, 3) * 2.0 ** 122).to(dtype)
+    check_attend(q, cache, cache, table, lengths, softmax_scale=2.0 ** -9)
+
+
+@pytest.mark.parametrize("Q,G", [(1, 1), (1, 40), (5, 9), (30, 3), (70, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_attend_v_scales_far_apart(Q, G, dtype):
+    """Every page weighs alike, their V differ: some all zeros (the least scale),
+    some far larger, some smaller.  The softmax's sum must count them all."""
+    lens = (330, 96 + Q, 320, 200, 17 + Q)
+    q, cache, _, table, lengths = attend_case(5, Q, 1, G, 64, 16, lens, E4M3, dtype, seed=Q + 3 * G)
+    cache.k_scale.mul_(2.0 ** -6)
+    cache.v_scale.fill_(2.0 ** -8)
+    for j in range(table.shape[1]):
+        if j % 3 == 1:
+            for b in (0, 1, 4):  # zeros among others
+                cache.v_cache.view(torch.uint8)[int(table[b, j])] = 0
+                cache.v_scale[int(table[b, j])] = kv8_layout.LEAST_SCALE
+        cache.v_scale[int(table[2, j])] = 2.0 ** ((j % 5 - 2) * 7 - 8)
+        if j > 7:
+            cache.v_scale[int(table[3, j])] = 2.0 ** -70
+    for b in range(5):
+        row = slice(b, b + 1)
+        check_attend(q[row], cache, cache, table[row], lengths[row])
+    check_attend(q, cache, cache, table, lengths)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("down", [118, 90])
+def test_attend_tiny_v(dtype, down):
+    q, cache, _, table, lengths = attend_case(2, 3, 2, 5, 64, 16, (70, 300), INT8, dtype, seed=14)
+    cache.v_scale.mul_(2.0 ** (8 - down))
+    check_attend(q, cache, cache, table, lengths)
+
+
+@pytest.mark.parametrize("Q,dtype", [(1, BF16), (1, F32), (20, BF16), (70, BF16)])
+def test_attend_v_scales_that_change_late_in_a_part(Q, dtype):
+    """Parts of more tiles than are looked up at once, V scales far apart from the
+    270th tile on: sums begun one way are carried on the other and joined."""
+    H, D, page, n = 32, 32, 256, 160000
+    pool, blocks = 24, -(-n // page)
+    cache = filled(pool, H, page, D, E4M3, seed=15, spread=0)
+    cache.k_scale.mul_(2.0 ** -6)
+    cache.v_cache.view(torch.uint8)[20:22] = 0
+    cache.v_scale[20:22] = kv8_layout.LEAST_SCALE
+    cache.v_scale[22:] *= 2.0 ** 20
+    table = (torch.arange(blocks) % 20).view(1, blocks).to(torch.int32)
+    for tile in range(270, 300, 4):
+        table[0, tile // 4] = 20 + tile // 4 % 4
+    lengths = torch.tensor([n], dtype=torch.int32)
+    q = torch.randn(1, Q, H, D, generator=gen(16)).to(dtype)
+    dev = to_gpu(cache)
+    got = native.kv8_decode_forward(q.to(DEV), *dev, table.to(DEV), lengths.to(DEV))
+    k, v = native.kv8_read(*dev, table.to(DEV), lengths.to(DEV), n, dtype=F32)
+    sees = n - Q + 1 + torch.arange(Q, device=DEV)
+    hidden = torch.arange(n, device=DEV)[None] >= sees[:, None]
+    for h in range(0, H, 5):
+        kh, vh, qh = k[0, h].double(), v[0, h].double(), q[0, :, h].to(DEV).double()
+        s = qh @ kh.T.contiguous() * D ** -0.5
+        p = torch.softmax(s.masked_fill(hidden, -float("inf")), -1)
+        size = (qh.abs() @ kh.abs().T.contiguous()).max(-1).values * D ** -0.5
+        want, mass = p @ vh, p @ vh.abs()
+        close(got[0, :, h], want.cpu().numpy(), mass.cpu().numpy(), size.cpu().numpy(), n, peak_of(cache))
 
 
 def test_attend_nan_and_infinite_inputs_stay_in_their_row():

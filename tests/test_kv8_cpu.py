@@ -100,8 +100,8 @@ def test_workspace_sizes(lib):
     assert f(2, -1, 1, 8, 8, 128, 64, 8) == f(2, 1, 1, 8, 0, 128, 64, 8) == f(2, 0, 1, 8, 8, 128, 64, 8) == 0
     assert g(2, 1, 8, 0, 128, 8, 64) == g(2, 1, 8, 8, 128, -8, 64) == g(2, 1, 8, 8, 128, 0, 64) == 0
     assert f(2, 1, 1, 8, 8, 128, 64, 16) == 0  # 1024 tokens: one part a sequence, nothing to join
-    # parts of at least 4 tiles of 64 tokens: 32 for 8192 tokens, each a row of 128 values, a maximum and a sum
-    assert f(2, 1, 1, 8, 8, 128, 64, 128) == 32 * 8 * 130 * 4
+    # parts of at least 4 tiles of 64 tokens: 32 for 8192 tokens, each a row of 128 values, two maxima and a sum (in four)
+    assert f(2, 1, 1, 8, 8, 128, 64, 128) == 32 * 8 * 132 * 4
     assert f(2, big, big, big, 1, 128, 64, big) == 0 and g(2, big, big, 1, 128, big, big) == 0
     assert f(0, 4, 50, 64, 8, 256, 256, 4096) > 0 and g(2, 1, 8, 8, 128, 64, 64) > 0
 
