@@ -4,6 +4,8 @@ over listed chunks, against the 64-bit restatement in oracle/kv8.py.
 Bytes and scales are compared for equality: with power-of-two scales the written
 byte is one rounding of an exact quotient.  Attention is held to a bound per
 value, out of what is rounded on the way to it (see ``bound``)."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -431,6 +433,26 @@ def test_attend_v_scales_far_apart(Q, G, dtype):
     check_attend(q, cache, cache, table, lengths)
 
 
+@pytest.mark.parametrize("dtype,G", [(BF16, 3), (F32, 2), (BF16, 80)])
+def test_attend_scales_that_are_no_powers_of_two(dtype, G):
+    q, cache, _, table, lengths = attend_case(3, 1, 2, G, 64, 16, (70, 300, 16), E4M3, dtype, seed=17)
+    for scale in cache[2:]:
+        scale.mul_(0.6 + torch.rand(scale.shape, generator=gen(18)))
+    check_attend(q, cache, cache, table, lengths)
+
+
+def test_attend_a_batch_of_more_sequences_than_lanes():
+    """Parts are found by a wavefront 64 sequences at a time."""
+    B = 150
+    lens = tuple(int(x) for x in torch.randint(0, 1300, (B,), generator=gen(19)))
+    for Q, n in ((1, lens), (1, (513,) * B), (35, lens)):
+        q, cache, dirty, table, lengths = attend_case(B, Q, 1, 2, 32, 64, n, E4M3, BF16, seed=20)
+        got = native.kv8_decode_forward(q.to(DEV), *to_gpu(cache), table.to(DEV), lengths.to(DEV))
+        rows = list(range(0, B, 7)) + [63, 64, 65, 127, 128, 149]
+        want, mass, size = plain.attend(q[rows], cache, table[rows], lengths[rows])
+        close(got[rows], want, mass, size, max(n), peak_of(cache))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("down", [118, 90])
 def test_attend_tiny_v(dtype, down):
@@ -594,6 +616,17 @@ def test_csa_many_heads_share_a_list(G, fmt, dtype):
     check_csa(q, cache, dirty, table, lengths, chunks, 36)
 
 
+@pytest.mark.parametrize("G", [1, 20, 70])
+def test_csa_of_pages_of_zeros_among_others(G):
+    q, cache, _, table, lengths = attend_case(2, 1, 1, G, 64, 16, (300, 77), E4M3, BF16, seed=G)
+    cache.k_scale.mul_(2.0 ** -6)
+    for b, j in ((0, 1), (0, 4), (1, 0), (1, 2)):
+        cache.v_cache.view(torch.uint8)[int(table[b, j])] = 0
+        cache.v_scale[int(table[b, j])] = kv8_layout.LEAST_SCALE
+    chunks = torch.tensor([[[3, 0, 1, 2, 5]], [[1, 0, 2, 2, -1]]], dtype=torch.int32)
+    check_csa(q, cache, cache, table, lengths, chunks, 32)
+
+
 @pytest.mark.parametrize("D", [32, 64, 96, 160, 192, 224, 256])
 @pytest.mark.parametrize("fmt,dtype", [(E4M3, BF16), (INT8, F16)])
 def test_attend_many_rows_of_every_head_size(D, fmt, dtype):
@@ -751,6 +784,30 @@ def test_results_do_not_change_from_call_to_call():
         assert torch.equal(first, native.kv8_decode_forward(*args))
 
 
+def test_calls_of_two_host_threads_on_one_stream_and_on_two():
+    q, cache, _, table, lengths = attend_case(3, 2, 2, 4, 64, 64, (5000, 900, 4097), E4M3, BF16, seed=22)
+    args = (*to_gpu(cache), table.to(DEV), lengths.to(DEV))
+    qs = [q.to(DEV), (q * 0.5).to(DEV)]
+    want = [native.kv8_decode_forward(x, *args) for x in qs]
+    torch.cuda.synchronize()
+    for streams in ([torch.cuda.current_stream()] * 2, [torch.cuda.Stream(), torch.cuda.Stream()]):
+        got = [[], []]
+
+        def calls(i):
+            with torch.cuda.stream(streams[i]):
+                for _ in range(20):
+                    got[i].append(native.kv8_decode_forward(qs[i], *args))
+                streams[i].synchronize()
+
+        threads = [threading.Thread(target=calls, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for i in range(2):
+            assert len(got[i]) == 20 and all(torch.equal(x, want[i]) for x in got[i])
+
+
 # ---------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------
@@ -786,6 +843,9 @@ def test_refusals():
     refused("cache's head_dim", att, q[..., :32].contiguous(), k, v, ks, vs, table, n)
     refused("unsupported dtype", att, q.double(), k, v, ks, vs, table, n)
     refused("q must be \\[", att, q[0], k, v, ks, vs, table, n)
+    odd = torch.zeros(q.numel() + 1, dtype=BF16, device=DEV)[1:].view(q.shape)
+    refused("16-byte aligned", att, odd, k, v, ks, vs, table, n)
+    refused("rows overlap", att, q, k, v, ks, vs, table[:1].expand(2, 2), n)
     csa = native.kv8_csa_decode_forward
     ids = torch.zeros(2, 2, 1, dtype=torch.int32, device=DEV)
     refused("q must be \\[", csa, q.unsqueeze(1), k, v, ks, vs, table, n, ids, 16)
