@@ -394,6 +394,12 @@ template <int D, int NP, int NT, bool kStream>
 constexpr int kKv8Blocks =
     D / 4 * (2 + NT) + NP * NT * D / 8 + 16 * NT + 8 * NP * NT <= (kStream ? 180 : 190) ? 2 : 1;
 
+// Bound by the read stream where there are tokens enough: 32 x 32768 tokens, 8 heads of
+// 128, 2.15 GB, 322 us (6.7 TB/s); 16 ragged ones of 4 rows 75 (5.7).  A wavefront keeps a
+// tile's K and V (16 KB at heads of 128) in flight while it works on the one before, two
+// workgroups a CU 128 KB.  1 x 8192 tokens take 9 us: lengths, table, scales and the tile,
+// a round trip each.
+//
 // kStream: no other wavefront reads a tile (one over the rows), and its loads go
 // past the caches: 32 x 32768 tokens 370 us without and 344 with (6.2 TB/s), 16 ragged
 // 78.6 / 73.4, 32 rows over 8 x 16384 tokens 59 / 54, of 192 84 / 77 (of 64 27 / 28);
@@ -841,8 +847,10 @@ __global__ __launch_bounds__(kKv8Threads, (kKv8Blocks<D, kF32 ? 3 : 1, NT, kStre
 // queries over 16384 tokens, heads 32 / 8 of 128, 271 GFLOP: the kernel above with
 // 32 rows a wavefront 329 us; 32x32x16 and shared operands, phase after phase, 337;
 // interleaved 313; eight wavefronts instead of four 278 (972 TFLOP/s; a library
-// product of 8192^3 in f16 reaches 1250).  What is left: writing operands to LDS
-// 47 us, reading them 20, the loads 22, exponentials 20.
+// product of 8192^3 in f16 reaches 1250); NaN bytes and scales far apart 284.  By
+// counters a SIMD's matrix instructions take 124 us and its vector instructions 146,
+// with little overlap.  Taken out one at a time, writing operands to LDS is 47 us,
+// reading them 20, the loads 22, exponentials 20.
 //
 // Lane l holds row n = l % 32; its half g = l / 32 the tokens of sub-block g of
 // each 32 of a tile: row 8b + 4g + j of a K tile is token 4b + j of sub-block g,

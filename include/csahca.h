@@ -378,7 +378,8 @@ int csahca_kv8_write(const void* k, const void* v, int dtype, int64_t k_stride_b
 
 /* Reads tokens back: k_out, v_out [batch, kv_heads, max_tokens, head_dim] hold
  * positions start[b] + n (start NULL: 0) as byte * scale, rounded once to
- * dtype; 0 at positions outside [0, lengths[b]) and on skipped pages. */
+ * dtype; 0 at positions outside [0, lengths[b]) and on skipped pages.  k_out and
+ * v_out are 16-byte aligned. */
 int csahca_kv8_read(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int format,
                     int64_t num_pages, int64_t page_size, const int32_t* block_table, int64_t blocks,
                     int64_t table_stride, const int32_t* start, const int32_t* lengths, void* k_out,
@@ -394,7 +395,8 @@ size_t csahca_kv8_decode_workspace_bytes(int dtype, int64_t batch, int64_t queri
  * head h reads K/V head h / (heads / kv_heads).  With n = lengths[b] (int32,
  * clamped to [0, blocks * page_size]), query i of `queries` attends to tokens
  * [0, n - queries + 1 + i): the queries are the last tokens of the sequence.
- * out = softmax(softmax_scale q.k) V, 0 where nothing is attended to. */
+ * out = softmax(softmax_scale q.k) V, 0 where nothing is attended to; scores are
+ * fp32 numbers.  q and out are 16-byte aligned, as is the workspace. */
 int csahca_kv8_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t queries, int64_t heads,
                               int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
                               const float* k_scale, const float* v_scale, int format, int64_t num_pages,
@@ -410,7 +412,8 @@ size_t csahca_kv8_csa_decode_workspace_bytes(int dtype, int64_t batch, int64_t h
  * chunk_indices [batch, kv_heads, top_k] (int32 or int64), one list for the
  * heads that share a K/V head.  Chunk c holds tokens [c * chunk_size,
  * (c + 1) * chunk_size); ids < 0 and tokens at or past lengths[b] are skipped,
- * a chunk listed twice counts twice; 0 when no token is left. */
+ * a chunk listed twice counts twice; 0 when no token is left.  Alignment as
+ * above. */
 int csahca_kv8_csa_decode_forward(const void* q, void* out, int dtype, int64_t batch, int64_t heads,
                                   int64_t kv_heads, int64_t head_dim, const void* k_cache, const void* v_cache,
                                   const float* k_scale, const float* v_scale, int format, int64_t num_pages,
