@@ -122,7 +122,8 @@ Split split_of(int dtype, int64_t batch, int64_t rows, int64_t kv_heads, int64_t
   const int64_t target = int64_t{1} << (list ? s.even_log2 : s.ragged_log2);
   const int64_t lanes = kv_heads * s.row_groups;
   if (list) {
-    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(ceil_div(tiles * batch * lanes, target), s.min_tiles), round) * round);
+    const int64_t per = batch * lanes >= target ? tiles : ceil_div(tiles * batch * lanes, target);
+    s.min_tiles = static_cast<int>(ceil_div(std::max<int64_t>(per, s.min_tiles), round) * round);
     s.parts = batch * ceil_div(tiles, s.min_tiles);
   } else {
     s.parts = std::min(target / lanes + batch, batch * std::max<int64_t>(ceil_div(tiles, s.min_tiles), 1));
@@ -142,6 +143,7 @@ int attend(Kv8Attend a, int format, int64_t tiles, void* workspace, size_t works
                  "too many query rows in one call");
   if (s.joined && (workspace == nullptr || workspace_bytes < workspace_of(s, a.c.kv_heads, a.rows, a.c.head_dim)))
     return fail(CSAHCA_ERR_WORKSPACE, "workspace too small for kv8 decode");
+  CSAHCA_REQUIRE(!s.joined || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be 16-byte aligned");
   const int64_t brows = int64_t{a.rows} * a.c.kv_heads, lanes = kKv8Threads / (a.c.head_dim / 4);
   a.join_lanes = static_cast<int32_t>(std::min(lanes, ceil_div(s.parts / a.batch, 4)));
   const int64_t join_grid = ceil_div(brows, lanes / a.join_lanes) * a.batch;

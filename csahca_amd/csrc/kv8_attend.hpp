@@ -144,7 +144,7 @@ __device__ __forceinline__ int32_t kv8_part_size(const Kv8Attend& a, int32_t* mi
   for (int d = 32; d >= 1; d /= 2) most = max(most, __float_as_int(xor_lanes(__int_as_float(most), d)));
   const int log2 = static_cast<int64_t>(most) * a.batch <= total + total / 8 ? a.even_log2 : a.ragged_log2;
   const int64_t per = (total * a.c.kv_heads * a.row_groups + (int64_t{1} << log2) - 1) >> log2;
-  return (max(a.min_tiles, static_cast<int32_t>(per)) + a.round - 1) & -a.round;
+  return (max(a.min_tiles, static_cast<int32_t>(min(per, int64_t{1} << 30))) + a.round - 1) & -a.round;
 }
 
 // The part of index `part` over all sequences, each of which has at least one

@@ -110,6 +110,22 @@ def test_missing_workspace_is_reported(lib):
     assert _attend(lib, blocks=128, tstride=128) == 2 and "workspace too small" in _error(lib)
     assert _csa(lib, top_k=64) == 2 and "workspace too small" in _error(lib)
     assert _attend(lib, q=8) == 1 and "16-byte aligned" in _error(lib)
+    enough = dict(wsb=1 << 60)
+    assert _attend(lib, blocks=128, tstride=128, ws=8, **enough) == 1 and "workspace must be 16-byte" in _error(lib)
+    assert _csa(lib, top_k=64, ws=24, **enough) == 1 and "workspace must be 16-byte" in _error(lib)
+
+
+def test_calls_beyond_a_launch_are_refused(lib):
+    """Grids of 2^32 threads and more, and sizes whose products pass 32 bits on the way."""
+    huge = dict(ws=16, wsb=1 << 62)
+    assert _attend(lib, B=1 << 25, blocks=128, tstride=128, **huge) == 1 and "too many query rows" in _error(lib)
+    assert _write(lib, B=1 << 22, H=4) == 1 and "too many tokens" in _error(lib)
+    assert _write(lib, B=1 << 14, N=1 << 20) == 1 and "too many tokens" in _error(lib)
+    assert _read(lib, B=1 << 20, N=1 << 20) == 1 and "too many tokens" in _error(lib)
+    assert _csa(lib, B=(1 << 31) - 1, heads=65534, top_k=1 << 20, **huge) == 1 and "too many query rows" in _error(lib)
+    g = lib.csahca_kv8_csa_decode_workspace_bytes
+    # a list is never divided further than it is long, however many sequences there are
+    assert g(2, (1 << 31) - 1, 64, 32, 128, 1 << 20, 64) == 0 and g(2, 1 << 20, 8, 8, 128, 1 << 20, 64) == 0
 
 
 def test_binding_rejects_cpu_tensors():
